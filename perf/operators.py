@@ -221,7 +221,7 @@ def _plan(case, s):
                                       case["cols"], types[case["type"]], EPS, residual_grads=each(s["arriving"]),
                                       send_grads=list(s["dsend"]) if "dsend" in s else None,
                                       weight_grads=list(s["dweight"]), workspace=s["workspace"],
-                                      residual_dtype=types[case["stream"]], grad_stride=case["cols"] + case["gap"])
+                                      residual_dtype=types[case["stream"]], send_stride=case["cols"] + case["gap"])
     offsets, _ = _places(case)
     lengths = _lengths(case)
     views = lambda t: [t[at:at + k] for at, k in zip(offsets, lengths)]  # noqa: E731
