@@ -361,6 +361,154 @@ MRV_API int mrv_comm_group_end(mrv_comm* comm);
 MRV_API int mrv_reduce_to_root(const void* const* sendbuffs, void* recvbuff_root, uint32_t nranks, size_t len,
                                int dtype, int op, int order, uint32_t root, void* stream);
 
+/* ---- folds with an epilogue ------------------------------------------------------------------ */
+
+/*
+ * No counterparts in the reference.  What a tensor- or data-parallel model does with a sum right behind its
+ * reduction, in the pass that makes the sum.  For all of these:
+ *   - ranks are summed in rank order 0 .. N-1 in 32 bits and every result is rounded once, when it is stored; the
+ *     same call gives the same bits every time;
+ *   - the calls only launch kernels on `stream` (they may be captured into a graph) and keep nothing of a call;
+ *   - an output may be exactly the input it replaces (same address, row stride and element size) where that is said
+ *     below; any other overlap of an output with an input or another output is rejected;
+ *   - device pointers have to be multiples of their element size, no more; rows may start anywhere and lie any
+ *     distance apart that is not less than their length.
+ * Two element types besides MegRay's are known to these calls alone:
+ */
+enum {
+    MRV_BFLOAT16 = 32,
+    MRV_FLOAT8_E4M3 = 33  /* 4 exponent bits, 3 mantissa bits, largest value 448, no infinities */
+};
+
+/*
+ * The norm behind a fold of partial activations (`dtype`: FLOAT16, MRV_BFLOAT16 or FLOAT32):
+ *   h = residual + sum over k of sendbuffs[k],   y = h / sqrt(mean(h * h) + eps) * weight     (mean over a row)
+ * collective MRV_ALL_REDUCE: the buffers hold `rows` rows; every rank's residual_outs / outs get all of h / y.  A
+ *   residual is replicated in such a model, so one copy is read: residuals[0], any rank's.
+ * collective MRV_REDUCE_SCATTER: sendbuffs[k] hold nranks * rows rows; residuals[r], residual_outs[r] and outs[r] are
+ *   rank r's `rows` rows.
+ * `residuals` null: h is the sum alone.  `residual_outs` null: h is not stored.  residual_dtype (of both): dtype or
+ * FLOAT32.  weight_dtype: dtype or FLOAT32.
+ * out_dtype: dtype, or INT8 / MRV_FLOAT8_E4M3: then scales[r] (one float per row of outs[r]) get
+ *   max(max |y|, 2^-100) / Q over the row and outs round(y / scale) to nearest even, Q = 127 / 448; a row with a value that is not
+ *   finite gets the scale NaN and the codes 0 / NaN.
+ * Strides are elements from one row to the next, 0 for cols.  cols >= 1; rows may be 0.
+ * outs[r] may be sendbuffs[r] (reduce_scatter: the place of rank r's own rows in it) and residual_outs[r] may be residuals[r] (all_reduce: residuals[0], for one r).
+ */
+typedef struct mrv_rms_norm_call {
+    const void* const* sendbuffs;
+    const void* const* residuals;
+    const void* weight;
+    void* const* residual_outs;
+    void* const* outs;
+    float* const* scales;
+    size_t rows, cols;
+    size_t send_stride, residual_stride, residual_out_stride, out_stride;
+    uint32_t nranks;
+    int dtype, residual_dtype, weight_dtype, out_dtype;
+    float eps;
+} mrv_rms_norm_call;
+MRV_API int mrv_rms_norm(int collective, const mrv_rms_norm_call* call, void* stream);
+
+/*
+ * Its backward.  sendbuffs[k] (`dtype`) hold rank k's partial gradients of y, laid out as the forward's sendbuffs; `hiddens` (residual_dtype) the
+ * h that the forward stored, `residual_grads` (residual_dtype, null: none) the gradient that arrives at h from elsewhere: one
+ * copy, entry 0 (all_reduce), or rank r's rows (reduce_scatter).  With g = sum over k of sendbuffs[k], r = 1 / sqrt(mean(h * h) + eps):
+ *   dh = r * g * weight - h * r^3 * mean(g * weight * h) + residual_grad
+ *   dweight = sum over rows of g * h * r
+ * dh is the gradient of the residual and of every rank's sendbuff of the forward: it goes to residual_out_grads
+ * (residual_dtype) and / or send_grads (dtype), either may be null, to every rank (all_reduce) or rank r's rows to rank r.
+ * weight_grads (null: not wanted): `cols` floats per rank, over all rows (all_reduce) or the rank's own (reduce_scatter);
+ * they need `workspace`, device memory of mrv_rms_norm_backward_workspace() bytes, aligned to 4 and not used by another call at the
+ * same time.  send_grads[r] may be sendbuffs[r] (reduce_scatter: its own rows there); residual_out_grads[r] may be residual_grads[r] or hiddens[r]
+ * (all_reduce: entry 0, for one r).
+ */
+typedef struct mrv_rms_norm_backward_call {
+    const void* const* sendbuffs;
+    const void* const* hiddens;
+    const void* const* residual_grads;
+    const void* weight;
+    void* const* residual_out_grads;
+    void* const* send_grads;
+    float* const* weight_grads;
+    void* workspace;
+    size_t workspace_bytes;
+    size_t rows, cols;
+    size_t send_stride, hidden_stride, residual_grad_stride, residual_out_grad_stride, send_grad_stride;
+    uint32_t nranks;
+    int dtype, residual_dtype, weight_dtype;
+    float eps;
+} mrv_rms_norm_backward_call;
+MRV_API int mrv_rms_norm_backward(int collective, const mrv_rms_norm_backward_call* call, void* stream);
+MRV_API int mrv_rms_norm_backward_workspace(int collective, uint32_t nranks, size_t rows, size_t cols, size_t* bytes);
+
+/* The same calls planned once and launched many times, as mrv_plan_create does for the plain collectives. */
+typedef struct mrv_norm_plan mrv_norm_plan;
+MRV_API int mrv_rms_norm_plan_create(int collective, const mrv_rms_norm_call* call, mrv_norm_plan** plan);
+MRV_API int mrv_rms_norm_backward_plan_create(int collective, const mrv_rms_norm_backward_call* call, mrv_norm_plan** plan);
+MRV_API int mrv_norm_plan_launch(const mrv_norm_plan* plan, void* stream);
+MRV_API size_t mrv_norm_plan_launch_count(const mrv_norm_plan* plan);
+MRV_API void mrv_norm_plan_destroy(mrv_norm_plan* plan);
+
+/*
+ * AdamW over many tensors at once, on gradients that are still apart: every rank's gradients are read and summed in
+ * the step itself, and the new parameters are written to every rank.  mrv_adamw_create checks the tensors and keeps their addresses in
+ * a table in device memory (it allocates and copies, synchronously); the tensors have to stay where they are until
+ * mrv_adamw_destroy, which frees the table: no call on the handle may still be running then.
+ *   grads[k * ntensors + t], params[k * ntensors + t]: rank k's tensor t, lens[t] elements of grad_dtype / param_dtype
+ *     (FLOAT16, MRV_BFLOAT16, FLOAT32).  grad_ranks and param_ranks (1 .. 32) may differ: gradients that were reduced
+ *     before have one rank.  lens[t] may be 0 (the pointers are not read then).
+ *   masters[t]: the 32-bit parameters the step works on; null where param_dtype is FLOAT32: then params[0 * ntensors + t].
+ *   exp_avgs[t], exp_avg_sqs[t]: the running means m and v.  state_dtype FLOAT32: floats.  MRV_FLOAT8_E4M3: codes with
+ *     a float scale for each 256 elements from the tensor's start (the last block may be shorter) in exp_avg_scales[t] and exp_avg_sq_scales[t]:
+ *     scale = max(max |x|, 2^-100) / 448 over the block, code = round(x / scale); the second holds x = sqrt(v), and
+ *     a value above zero gets at least the smallest code (2^-9), so that no denominator is lost.  Zeroed codes and scales are
+ *     a valid beginning.
+ *   weight_decays[t] (null: 0).
+ * A handle without params (null) serves mrv_adamw_grad_norm alone.
+ */
+typedef struct mrv_adamw mrv_adamw;
+typedef struct mrv_adamw_tensors {
+    size_t ntensors;
+    const size_t* lens;
+    const void* const* grads;
+    void* const* params;
+    float* const* masters;
+    void* const* exp_avgs;
+    void* const* exp_avg_sqs;
+    float* const* exp_avg_scales;
+    float* const* exp_avg_sq_scales;
+    const float* weight_decays;
+    uint32_t grad_ranks, param_ranks;
+    int grad_dtype, param_dtype, state_dtype;
+} mrv_adamw_tensors;
+MRV_API int mrv_adamw_create(const mrv_adamw_tensors* tensors, mrv_adamw** handle);
+MRV_API void mrv_adamw_destroy(mrv_adamw* handle);
+
+/*
+ * The norm of all folded gradients, g = grad_scale * sum over k of grads[k]:
+ *   out[0] = sqrt(sum of g * g),   out[1] = min(1, max_norm / (out[0] + 1e-6)), or NaN where the norm is not finite.
+ * Squares are summed in 64 bits.  `out` is device memory of mrv_adamw_norm_floats() floats, aligned to 8; what follows
+ * out[1] is scratch.  Calls that may run at the same time need an `out` each.
+ */
+MRV_API size_t mrv_adamw_norm_floats(const mrv_adamw* handle);
+MRV_API int mrv_adamw_grad_norm(const mrv_adamw* handle, float grad_scale, float max_norm, float* out, void* stream);
+
+/*
+ * One step, with g = grad_scale * *clip * sum over k of grads[k] (clip: a float in device memory, out + 1 of the call above say; null: 1):
+ *   m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g g,
+ *   p = p (1 - lr weight_decay) - lr (m / (1 - beta1^step)) / (sqrt(v / (1 - beta2^step)) + eps)
+ * in 32 bits; params get p rounded to their type.  A step whose *clip is not finite changes nothing.  `step` counts from 1.  The
+ * numbers are arguments of the launch: a step captured into a graph repeats them.
+ */
+typedef struct mrv_adamw_step_args {
+    double lr, beta1, beta2, eps;
+    double grad_scale;
+    uint64_t step;
+    const float* clip;
+} mrv_adamw_step_args;
+MRV_API int mrv_adamw_step(const mrv_adamw* handle, const mrv_adamw_step_args* args, void* stream);
+
 /* The bootstrap client (include/megray/client.h:24-49), host memory only. */
 typedef struct mrv_client mrv_client;
 MRV_API int mrv_client_create(uint32_t nranks, uint32_t rank, mrv_client** client);

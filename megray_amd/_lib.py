@@ -23,6 +23,51 @@ class PlanRun(ctypes.Structure):
     ]
 
 
+_pp = ctypes.POINTER(ctypes.c_void_p)
+
+
+class RmsNormCall(ctypes.Structure):
+    """struct mrv_rms_norm_call"""
+    _fields_ = [
+        ("sendbuffs", _pp), ("residuals", _pp), ("weight", ctypes.c_void_p), ("residual_outs", _pp), ("outs", _pp),
+        ("scales", _pp), ("rows", ctypes.c_size_t), ("cols", ctypes.c_size_t), ("send_stride", ctypes.c_size_t),
+        ("residual_stride", ctypes.c_size_t), ("residual_out_stride", ctypes.c_size_t), ("out_stride", ctypes.c_size_t),
+        ("nranks", ctypes.c_uint32), ("dtype", ctypes.c_int), ("residual_dtype", ctypes.c_int),
+        ("weight_dtype", ctypes.c_int), ("out_dtype", ctypes.c_int), ("eps", ctypes.c_float),
+    ]
+
+
+class RmsNormBackwardCall(ctypes.Structure):
+    """struct mrv_rms_norm_backward_call"""
+    _fields_ = [
+        ("sendbuffs", _pp), ("hiddens", _pp), ("residual_grads", _pp), ("weight", ctypes.c_void_p),
+        ("residual_out_grads", _pp), ("send_grads", _pp), ("weight_grads", _pp), ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t), ("rows", ctypes.c_size_t), ("cols", ctypes.c_size_t),
+        ("send_stride", ctypes.c_size_t), ("hidden_stride", ctypes.c_size_t), ("residual_grad_stride", ctypes.c_size_t),
+        ("residual_out_grad_stride", ctypes.c_size_t), ("send_grad_stride", ctypes.c_size_t),
+        ("nranks", ctypes.c_uint32), ("dtype", ctypes.c_int), ("residual_dtype", ctypes.c_int),
+        ("weight_dtype", ctypes.c_int), ("eps", ctypes.c_float),
+    ]
+
+
+class AdamwTensors(ctypes.Structure):
+    """struct mrv_adamw_tensors"""
+    _fields_ = [
+        ("ntensors", ctypes.c_size_t), ("lens", ctypes.POINTER(ctypes.c_size_t)), ("grads", _pp), ("params", _pp),
+        ("masters", _pp), ("exp_avgs", _pp), ("exp_avg_sqs", _pp), ("exp_avg_scales", _pp), ("exp_avg_sq_scales", _pp),
+        ("weight_decays", ctypes.POINTER(ctypes.c_float)), ("grad_ranks", ctypes.c_uint32), ("param_ranks", ctypes.c_uint32),
+        ("grad_dtype", ctypes.c_int), ("param_dtype", ctypes.c_int), ("state_dtype", ctypes.c_int),
+    ]
+
+
+class AdamwStepArgs(ctypes.Structure):
+    """struct mrv_adamw_step_args"""
+    _fields_ = [
+        ("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double),
+        ("grad_scale", ctypes.c_double), ("step", ctypes.c_uint64), ("clip", ctypes.c_void_p),
+    ]
+
+
 # void (*mrv_bcast_fn)(char* data, size_t len, void* user)
 BCAST_FN = ctypes.CFUNCTYPE(None, ctypes.POINTER(ctypes.c_char), ctypes.c_size_t, ctypes.c_void_p)
 
@@ -120,6 +165,27 @@ def load():
     for name in ("mrv_reduce", "mrv_all_reduce", "mrv_reduce_scatter", "mrv_all_gather",
                  "mrv_all_to_all", "mrv_scatter", "mrv_gather", "mrv_broadcast", "mrv_chunk_partition",
                  "mrv_fold_order", "mrv_describe"):
+        getattr(L, name).restype = i32
+    L.mrv_rms_norm.argtypes = [i32, ctypes.POINTER(RmsNormCall), vp]
+    L.mrv_rms_norm_backward.argtypes = [i32, ctypes.POINTER(RmsNormBackwardCall), vp]
+    L.mrv_rms_norm_backward_workspace.argtypes = [i32, u32, sz, sz, ctypes.POINTER(sz)]
+    L.mrv_rms_norm_plan_create.argtypes = [i32, ctypes.POINTER(RmsNormCall), ctypes.POINTER(vp)]
+    L.mrv_rms_norm_backward_plan_create.argtypes = [i32, ctypes.POINTER(RmsNormBackwardCall), ctypes.POINTER(vp)]
+    L.mrv_norm_plan_launch.argtypes = [vp, vp]
+    L.mrv_norm_plan_launch_count.argtypes = [vp]
+    L.mrv_norm_plan_launch_count.restype = sz
+    L.mrv_norm_plan_destroy.argtypes = [vp]
+    L.mrv_norm_plan_destroy.restype = None
+    L.mrv_adamw_create.argtypes = [ctypes.POINTER(AdamwTensors), ctypes.POINTER(vp)]
+    L.mrv_adamw_destroy.argtypes = [vp]
+    L.mrv_adamw_destroy.restype = None
+    L.mrv_adamw_norm_floats.argtypes = [vp]
+    L.mrv_adamw_norm_floats.restype = sz
+    L.mrv_adamw_grad_norm.argtypes = [vp, ctypes.c_float, ctypes.c_float, vp, vp]
+    L.mrv_adamw_step.argtypes = [vp, ctypes.POINTER(AdamwStepArgs), vp]
+    for name in ("mrv_rms_norm", "mrv_rms_norm_backward", "mrv_rms_norm_backward_workspace", "mrv_rms_norm_plan_create",
+                 "mrv_rms_norm_backward_plan_create", "mrv_norm_plan_launch", "mrv_adamw_create", "mrv_adamw_grad_norm",
+                 "mrv_adamw_step"):
         getattr(L, name).restype = i32
     _lib = L
     return L

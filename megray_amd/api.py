@@ -48,6 +48,9 @@ class DType(enum.IntEnum):
     FLOAT32 = 7
     FLOAT64 = 8
     CHAR = 9
+    # element types of the folds with an epilogue (RmsNormPlan ... AdamWPlan) alone; every other call refuses them
+    BFLOAT16 = 32
+    FLOAT8_E4M3 = 33
 
 
 class ReduceOp(enum.IntEnum):
@@ -338,6 +341,215 @@ class CollectivePlan:
     def close(self):
         if self._h:
             _lib.load().mrv_plan_destroy(self._h)
+            self._h = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:  # at interpreter shutdown the modules this needs may be gone already
+            pass
+
+
+# ---------------------------------------------------------------------------------------------
+# folds with an epilogue: what a tensor- or data-parallel model does with a sum right behind its reduction
+
+def _optional_array(bufs, n, what):
+    if bufs is None:
+        return None
+    if len(bufs) != n:
+        raise MegRayError(Status.INVALID_ARGUMENT, f"{len(bufs)} {what}, {n} expected")
+    return _ptr_array(bufs)
+
+
+def _copies(collective, nranks):
+    """How many copies of a residual a call reads: it is replicated behind an all_reduce, every rank's own behind a
+    reduce_scatter."""
+    return 1 if int(collective) == Collective.ALL_REDUCE else nranks
+
+
+def _rms_norm_call(collective, sendbuffs, outs, weight, rows, cols, dtype, eps, residuals=None, residual_outs=None,
+                   scales=None, residual_dtype=None, weight_dtype=None, out_dtype=None, send_stride=0, residual_stride=0,
+                   residual_out_stride=0, out_stride=0):
+    n = len(sendbuffs)
+    pick = lambda t: int(dtype if t is None else t)  # noqa: E731
+    return _lib.RmsNormCall(
+        sendbuffs=_ptr_array(sendbuffs), residuals=_optional_array(residuals, _copies(collective, n), "residuals"),
+        weight=_ptr(weight), residual_outs=_optional_array(residual_outs, n, "residual outputs"),
+        outs=_optional_array(outs, n, "outputs"), scales=_optional_array(scales, n, "scale buffers"), rows=rows, cols=cols,
+        send_stride=send_stride, residual_stride=residual_stride, residual_out_stride=residual_out_stride,
+        out_stride=out_stride, nranks=n, dtype=int(dtype), residual_dtype=pick(residual_dtype),
+        weight_dtype=pick(weight_dtype), out_dtype=pick(out_dtype), eps=eps)
+
+
+def _rms_norm_backward_call(collective, sendbuffs, hiddens, weight, residual_out_grads, rows, cols, dtype, eps,
+                            residual_grads=None, send_grads=None, weight_grads=None, workspace=None, workspace_bytes=None,
+                            residual_dtype=None, weight_dtype=None, send_stride=0, hidden_stride=0, residual_grad_stride=0,
+                            residual_out_grad_stride=0, send_grad_stride=0):
+    n = len(sendbuffs)
+    pick = lambda t: int(dtype if t is None else t)  # noqa: E731
+    if workspace_bytes is None:
+        workspace_bytes = workspace.numel() * workspace.element_size() if hasattr(workspace, "numel") else 0
+    return _lib.RmsNormBackwardCall(
+        sendbuffs=_ptr_array(sendbuffs), hiddens=_optional_array(hiddens, _copies(collective, n), "hidden states"),
+        residual_grads=_optional_array(residual_grads, _copies(collective, n), "residual gradients"), weight=_ptr(weight),
+        residual_out_grads=_optional_array(residual_out_grads, n, "residual gradient outputs"),
+        send_grads=_optional_array(send_grads, n, "send gradients"),
+        weight_grads=_optional_array(weight_grads, n, "weight gradients"), workspace=_ptr(workspace),
+        workspace_bytes=workspace_bytes, rows=rows, cols=cols, send_stride=send_stride, hidden_stride=hidden_stride,
+        residual_grad_stride=residual_grad_stride, residual_out_grad_stride=residual_out_grad_stride,
+        send_grad_stride=send_grad_stride, nranks=n, dtype=int(dtype), residual_dtype=pick(residual_dtype),
+        weight_dtype=pick(weight_dtype), eps=eps)
+
+
+def all_reduce_rms_norm(sendbuffs, outs, weight, rows, cols, dtype, eps, stream=None, **more):
+    """h = residual + sum of sendbuffs, outs = h / sqrt(mean(h * h) + eps) * weight, both to every rank (mrv_rms_norm).
+
+    Optional: residuals=[one copy], residual_outs (h, one per rank), scales (one per rank, with out_dtype INT8 or
+    FLOAT8_E4M3), residual_dtype, weight_dtype, out_dtype (default: dtype), and the strides from row to row in elements:
+    send_stride, residual_stride, residual_out_stride, out_stride."""
+    call = _rms_norm_call(Collective.ALL_REDUCE, sendbuffs, outs, weight, rows, cols, dtype, eps, **more)
+    _check(_lib.load().mrv_rms_norm(int(Collective.ALL_REDUCE), call, _stream(stream)))
+
+
+def reduce_scatter_rms_norm(sendbuffs, outs, weight, rows, cols, dtype, eps, stream=None, **more):
+    """The same behind a reduce_scatter: rank r gets `rows` rows, r * rows and following, of the fold; residuals, residual_outs,
+    outs and scales are each rank's own (mrv_rms_norm)."""
+    call = _rms_norm_call(Collective.REDUCE_SCATTER, sendbuffs, outs, weight, rows, cols, dtype, eps, **more)
+    _check(_lib.load().mrv_rms_norm(int(Collective.REDUCE_SCATTER), call, _stream(stream)))
+
+
+def all_reduce_rms_norm_backward(sendbuffs, hiddens, weight, residual_out_grads, rows, cols, dtype, eps, stream=None, **more):
+    """Backward of all_reduce_rms_norm: sendbuffs hold the ranks' partial gradients of its outs, hiddens=[one copy of h]
+    (mrv_rms_norm_backward).  residual_out_grads (or None) get the gradient of the residual and of every forward send buffer.
+
+    Optional: residual_grads=[one copy] (the gradient that arrives at h from elsewhere), send_grads (the same gradient
+    in `dtype`), weight_grads (cols floats per rank; they need workspace=, of rms_norm_backward_workspace() bytes), residual_dtype, weight_dtype, and the
+    strides send_stride, hidden_stride, residual_grad_stride, residual_out_grad_stride, send_grad_stride."""
+    call = _rms_norm_backward_call(Collective.ALL_REDUCE, sendbuffs, hiddens, weight, residual_out_grads, rows, cols, dtype, eps, **more)
+    _check(_lib.load().mrv_rms_norm_backward(int(Collective.ALL_REDUCE), call, _stream(stream)))
+
+
+def reduce_scatter_rms_norm_backward(sendbuffs, hiddens, weight, residual_out_grads, rows, cols, dtype, eps, stream=None, **more):
+    """Backward of reduce_scatter_rms_norm: hiddens, residual_grads and all outputs are each rank's own rows; weight_grads
+    are sums over the rank's rows (mrv_rms_norm_backward)."""
+    call = _rms_norm_backward_call(Collective.REDUCE_SCATTER, sendbuffs, hiddens, weight, residual_out_grads, rows, cols, dtype, eps, **more)
+    _check(_lib.load().mrv_rms_norm_backward(int(Collective.REDUCE_SCATTER), call, _stream(stream)))
+
+
+def rms_norm_backward_workspace(collective, nranks, rows, cols):
+    """Bytes of workspace a backward with weight gradients needs (mrv_rms_norm_backward_workspace)."""
+    size = ctypes.c_size_t(0)
+    _check(_lib.load().mrv_rms_norm_backward_workspace(int(collective), nranks, rows, cols, ctypes.byref(size)))
+    return size.value
+
+
+class _NormPlan:
+    def __init__(self, create, collective, call, keep):
+        self._h = ctypes.c_void_p()
+        self._keep = keep  # the buffers must outlive the plan
+        _check(create(int(collective), call, ctypes.byref(self._h)))
+        self._launch = _lib.load().mrv_norm_plan_launch
+
+    @property
+    def launch_count(self):
+        return _lib.load().mrv_norm_plan_launch_count(self._h)
+
+    def launch(self, stream=None):
+        status = self._launch(self._h, _stream(stream))
+        if status:
+            _check(status)
+
+    def close(self):
+        if self._h:
+            _lib.load().mrv_norm_plan_destroy(self._h)
+            self._h = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:  # at interpreter shutdown the modules this needs may be gone already
+            pass
+
+
+class RmsNormPlan(_NormPlan):
+    """all_reduce_rms_norm / reduce_scatter_rms_norm planned once and launched many times (mrv_rms_norm_plan_create): the same
+    arguments behind `collective`."""
+
+    def __init__(self, collective, sendbuffs, outs, weight, rows, cols, dtype, eps, **more):
+        call = _rms_norm_call(collective, sendbuffs, outs, weight, rows, cols, dtype, eps, **more)
+        super().__init__(_lib.load().mrv_rms_norm_plan_create, collective, call, (sendbuffs, outs, weight, more))
+
+
+class RmsNormBackwardPlan(_NormPlan):
+    """The backward calls planned once and launched many times (mrv_rms_norm_backward_plan_create)."""
+
+    def __init__(self, collective, sendbuffs, hiddens, weight, residual_out_grads, rows, cols, dtype, eps, **more):
+        call = _rms_norm_backward_call(collective, sendbuffs, hiddens, weight, residual_out_grads, rows, cols, dtype, eps, **more)
+        super().__init__(_lib.load().mrv_rms_norm_backward_plan_create, collective, call,
+                         (sendbuffs, hiddens, weight, residual_out_grads, more))
+
+
+class AdamWPlan:
+    """AdamW over many tensors whose gradients are still apart on the ranks (mrv_adamw_*).
+
+    grads[r][t]: rank r's gradient of tensor t, lengths[t] elements of grad_dtype; params[r][t] likewise, written by step().
+    masters[t]: the 32-bit parameters (None with FLOAT32 params: rank 0's are the masters).  exp_avgs, exp_avg_sqs: floats, or
+    with state_dtype FLOAT8_E4M3 codes with a float for each 256 elements in exp_avg_scales[t], exp_avg_sq_scales[t].
+    Without params a plan has grad_norm() alone.  The tensors must outlive the plan, and stay where they are."""
+
+    def __init__(self, grads, lengths, grad_dtype, params=None, param_dtype=None, masters=None, exp_avgs=None, exp_avg_sqs=None,
+                 state_dtype=DType.FLOAT32, exp_avg_scales=None, exp_avg_sq_scales=None, weight_decays=None):
+        self._h = ctypes.c_void_p()
+        self._keep = (grads, params, masters, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales)
+        n = len(lengths)
+
+        def ranks(lists, what):
+            if lists is None:
+                return None
+            if any(len(x) != n for x in lists):
+                raise MegRayError(Status.INVALID_ARGUMENT, f"every rank has {n} {what}")
+            return _ptr_array([t for x in lists for t in x])
+
+        if weight_decays is not None and len(weight_decays) != n:
+            raise MegRayError(Status.INVALID_ARGUMENT, f"{len(weight_decays)} weight decays for {n} tensors")
+        call = _lib.AdamwTensors(
+            ntensors=n, lens=(ctypes.c_size_t * max(n, 1))(*lengths), grads=ranks(grads, "gradients"), params=ranks(params, "parameters"),
+            masters=_optional_array(masters, n, "masters"), exp_avgs=_optional_array(exp_avgs, n, "running means"),
+            exp_avg_sqs=_optional_array(exp_avg_sqs, n, "running means of squares"),
+            exp_avg_scales=_optional_array(exp_avg_scales, n, "scale buffers"),
+            exp_avg_sq_scales=_optional_array(exp_avg_sq_scales, n, "scale buffers"),
+            weight_decays=None if weight_decays is None else (ctypes.c_float * max(n, 1))(*weight_decays),
+            grad_ranks=len(grads), param_ranks=0 if params is None else len(params), grad_dtype=int(grad_dtype),
+            param_dtype=int(grad_dtype if param_dtype is None else param_dtype), state_dtype=int(state_dtype))
+        _check(_lib.load().mrv_adamw_create(call, ctypes.byref(self._h)))
+        self._step = _lib.load().mrv_adamw_step
+        self._norm = _lib.load().mrv_adamw_grad_norm
+
+    @property
+    def norm_floats(self):
+        """Floats that grad_norm()'s `out` has to hold."""
+        return _lib.load().mrv_adamw_norm_floats(self._h)
+
+    def grad_norm(self, out, grad_scale=1.0, max_norm=float("inf"), stream=None):
+        """out[0] = the norm of grad_scale * the folded gradients, out[1] = min(1, max_norm / (norm + 1e-6)), NaN where the norm is
+        not finite; what follows is scratch (mrv_adamw_grad_norm)."""
+        status = self._norm(self._h, grad_scale, max_norm, _ptr(out), _stream(stream))
+        if status:
+            _check(status)
+
+    def step(self, lr, step, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, clip=None, stream=None):
+        """One AdamW step, number `step` (from 1 on), on grad_scale * clip * the folded gradients; clip: a float in device
+        memory (grad_norm()'s out[1:], say).  A step whose clip is not finite changes nothing (mrv_adamw_step)."""
+        if step < 1:
+            raise MegRayError(Status.INVALID_ARGUMENT, "step counts from 1")
+        args = _lib.AdamwStepArgs(lr=lr, beta1=beta1, beta2=beta2, eps=eps, grad_scale=grad_scale, step=step, clip=_ptr(clip))
+        status = self._step(self._h, args, _stream(stream))
+        if status:
+            _check(status)
+
+    def close(self):
+        if self._h:
+            _lib.load().mrv_adamw_destroy(self._h)
             self._h = ctypes.c_void_p()
 
     def __del__(self):

@@ -15,6 +15,7 @@
 #include "vrank_edges.h"
 #include "megray/hip_context.h"
 #include "vrank_engine.h"
+#include "vrank_fused.h"
 #include "vrank_kernels.h"
 #include "vrank_placement.h"
 #include "vrank_plan.h"
@@ -59,6 +60,9 @@ int guarded(F&& body) {
     } catch (const MegRay::Exception& e) {
         set_error(e.what());
         return int(MEGRAY_INVALID_ARGUMENT);
+    } catch (const HipFailure&) {
+        set_error("hip error while the handle was made");
+        return int(MEGRAY_HIP_ERR);
     } catch (const std::exception& e) {
         set_error(e.what());
         return int(MEGRAY_UNEXPECTED_ERR);
@@ -760,6 +764,119 @@ int mrv_client_allgather(mrv_client* client, const void* sendbuff, void* recvbuf
     return guarded([&] {
         need(client, "client is null");
         return client->client->allgather(sendbuff, recvbuff, sendlen);
+    });
+}
+
+}  // extern "C"
+
+// ---- folds with an epilogue --------------------------------------------------------------------
+
+struct mrv_norm_plan {
+    NormPlan plan;
+};
+
+struct mrv_adamw {
+    Adamw adamw;
+    explicit mrv_adamw(const mrv_adamw_tensors& tensors) : adamw(tensors) {}
+};
+
+extern "C" {
+
+int mrv_rms_norm(int collective, const mrv_rms_norm_call* call, void* stream) {
+    return guarded([&] {
+        need(call, "call is null");
+        NormPlan plan;
+        plan.plan_forward(collective, *call);
+        return plan.launch(as_stream(stream));
+    });
+}
+
+int mrv_rms_norm_backward(int collective, const mrv_rms_norm_backward_call* call, void* stream) {
+    return guarded([&] {
+        need(call, "call is null");
+        NormPlan plan;
+        plan.plan_backward(collective, *call);
+        return plan.launch(as_stream(stream));
+    });
+}
+
+int mrv_rms_norm_backward_workspace(int collective, uint32_t nranks, size_t rows, size_t cols, size_t* bytes) {
+    return guarded([&] {
+        need(bytes, "bytes is null");
+        *bytes = norm_backward_workspace(collective, nranks, rows, cols);
+        return MEGRAY_OK;
+    });
+}
+
+int mrv_rms_norm_plan_create(int collective, const mrv_rms_norm_call* call, mrv_norm_plan** plan) {
+    return guarded([&] {
+        need(plan, "plan is null");
+        *plan = nullptr;
+        need(call, "call is null");
+        std::unique_ptr<mrv_norm_plan> p(new mrv_norm_plan);
+        p->plan.plan_forward(collective, *call);
+        *plan = p.release();
+        return MEGRAY_OK;
+    });
+}
+
+int mrv_rms_norm_backward_plan_create(int collective, const mrv_rms_norm_backward_call* call, mrv_norm_plan** plan) {
+    return guarded([&] {
+        need(plan, "plan is null");
+        *plan = nullptr;
+        need(call, "call is null");
+        std::unique_ptr<mrv_norm_plan> p(new mrv_norm_plan);
+        p->plan.plan_backward(collective, *call);
+        *plan = p.release();
+        return MEGRAY_OK;
+    });
+}
+
+int mrv_norm_plan_launch(const mrv_norm_plan* plan, void* stream) {
+    return guarded([&] {
+        need(plan, "plan is null");
+        return plan->plan.launch(as_stream(stream));
+    });
+}
+
+size_t mrv_norm_plan_launch_count(const mrv_norm_plan* plan) {
+    return plan ? plan->plan.launch_count() : 0;
+}
+
+void mrv_norm_plan_destroy(mrv_norm_plan* plan) {
+    delete plan;
+}
+
+int mrv_adamw_create(const mrv_adamw_tensors* tensors, mrv_adamw** handle) {
+    return guarded([&] {
+        need(handle, "handle is null");
+        *handle = nullptr;
+        need(tensors, "tensors is null");
+        *handle = new mrv_adamw(*tensors);
+        return MEGRAY_OK;
+    });
+}
+
+void mrv_adamw_destroy(mrv_adamw* handle) {
+    delete handle;
+}
+
+size_t mrv_adamw_norm_floats(const mrv_adamw* handle) {
+    return handle ? handle->adamw.norm_floats() : 0;
+}
+
+int mrv_adamw_grad_norm(const mrv_adamw* handle, float grad_scale, float max_norm, float* out, void* stream) {
+    return guarded([&] {
+        need(handle, "handle is null");
+        return handle->adamw.grad_norm(grad_scale, max_norm, out, as_stream(stream));
+    });
+}
+
+int mrv_adamw_step(const mrv_adamw* handle, const mrv_adamw_step_args* args, void* stream) {
+    return guarded([&] {
+        need(handle, "handle is null");
+        need(args, "args is null");
+        return handle->adamw.step(*args, as_stream(stream));
     });
 }
 

@@ -1,0 +1,565 @@
+// Argument checks, planning and launching of the folds with an epilogue (vrank_fused.h).
+#include "vrank_fused.h"
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <new>
+
+#include "megray/hip_context.h"
+#include "vrank_kernels.h"
+
+namespace MegRay {
+namespace vrank {
+
+namespace {
+
+// ---- checks ----------------------------------------------------------------------------------
+
+size_t float_size(int dtype, const char* what) {
+    switch (dtype) {
+        case MEGRAY_FLOAT16:
+        case MRV_BFLOAT16: return 2;
+        case MEGRAY_FLOAT32: return 4;
+        default: MEGRAY_THROW(what);
+    }
+}
+
+void check_pointer(const void* p, size_t align, const char* null_text) {
+    if (!p) MEGRAY_THROW(null_text);
+    if (reinterpret_cast<uintptr_t>(p) % align) MEGRAY_THROW("a buffer does not lie on a multiple of its element size");
+}
+
+// Rows of a buffer: `rows` of `bytes` bytes, `stride` bytes apart.
+struct Rows {
+    uintptr_t at;
+    uint64_t rows, bytes, stride;
+    uint32_t elem;
+    uint64_t end() const { return rows ? at + (rows - 1) * stride + bytes : at; }
+};
+
+bool overlap(const Rows& a, const Rows& b) {
+    if (!a.rows || !b.rows || a.at >= b.end() || b.at >= a.end()) return false;
+    if (a.stride && a.stride == b.stride) {  // column ranges of one matrix lie between each other's rows
+        const uint64_t d = (b.at >= a.at ? b.at - a.at : a.stride - (a.at - b.at) % a.stride) % a.stride;
+        if (d >= a.bytes && d + b.bytes <= a.stride) return false;
+    }
+    return true;
+}
+
+bool same_place(const Rows& a, const Rows& b) {
+    return a.at == b.at && a.elem == b.elem && (a.stride == b.stride || a.rows == 1);
+}
+
+// Every output against every input and output.  `replaces[o]` is the input that output o may be, or -1.
+void check_rows(const std::vector<Rows>& outputs, const std::vector<int>& replaces, const std::vector<Rows>& inputs,
+                const std::vector<Rows>& replaced) {
+    for (size_t o = 0; o < outputs.size(); ++o) {
+        for (size_t p = o + 1; p < outputs.size(); ++p)
+            if (overlap(outputs[o], outputs[p])) MEGRAY_THROW("two outputs overlap");
+        for (size_t i = 0; i < inputs.size(); ++i) {
+            if (!overlap(outputs[o], inputs[i])) continue;
+            if (replaces[o] == int(i) && same_place(outputs[o], replaced[i])) continue;
+            MEGRAY_THROW("an output overlaps an input out of place");
+        }
+    }
+}
+
+struct Shape {
+    bool gathered;  // all_reduce
+    uint32_t nranks, cols, part_rows, rows;
+    size_t elem, stream_elem;
+    bool stream32, weight32;
+};
+
+constexpr uint64_t kMaxStride = uint64_t(1) << 40;
+
+uint64_t row_bytes(size_t stride, size_t cols, size_t elem) {
+    if (!stride) stride = cols;
+    if (stride < cols) MEGRAY_THROW("a row stride is less than the row's length");
+    if (stride > kMaxStride) MEGRAY_THROW("a row stride is out of range");
+    return uint64_t(stride) * elem;
+}
+
+void check_collective(int collective, uint32_t nranks) {
+    if (collective != MRV_ALL_REDUCE && collective != MRV_REDUCE_SCATTER)
+        MEGRAY_THROW("the norm stands behind an all_reduce or a reduce_scatter");
+    if (nranks < 1 || nranks > kMaxRanks) MEGRAY_THROW("nranks must be in [1, 32]");
+}
+
+// Rows of the fold and row lengths that the launches count in 32 bits (grids in lanes, too).
+void check_extent(uint64_t rows, uint64_t cols) {
+    if (cols < 1) MEGRAY_THROW("a row needs at least one element");
+    if (cols > (uint64_t(1) << 30)) MEGRAY_THROW("a row is too long");
+    if (rows >= (uint64_t(1) << 22)) MEGRAY_THROW("too many rows");
+}
+
+Shape check_shape(int collective, uint32_t nranks, size_t rows, size_t cols, int dtype, int residual_dtype, int weight_dtype, float eps) {
+    check_collective(collective, nranks);
+    Shape s;
+    s.gathered = collective == MRV_ALL_REDUCE;
+    s.nranks = nranks;
+    s.elem = float_size(dtype, "unknown dtype");
+    s.stream_elem = float_size(residual_dtype, "unknown residual dtype");
+    (void)float_size(weight_dtype, "unknown weight dtype");
+    if (residual_dtype != dtype && residual_dtype != MEGRAY_FLOAT32) MEGRAY_THROW("the residual's dtype is the sends' or FLOAT32");
+    if (weight_dtype != dtype && weight_dtype != MEGRAY_FLOAT32) MEGRAY_THROW("the weight's dtype is the sends' or FLOAT32");
+    s.stream32 = residual_dtype == MEGRAY_FLOAT32;
+    s.weight32 = weight_dtype == MEGRAY_FLOAT32;
+    if (!(eps >= 0.0f) || !std::isfinite(eps)) MEGRAY_THROW("eps must be finite and not negative");
+    if (rows >= (uint64_t(1) << 22)) MEGRAY_THROW("too many rows");
+    check_extent(s.gathered ? rows : uint64_t(rows) * nranks, cols);
+    s.cols = uint32_t(cols);
+    s.part_rows = uint32_t(rows);
+    s.rows = s.gathered ? s.part_rows : s.part_rows * nranks;
+    return s;
+}
+
+// ---- how a norm is laid out --------------------------------------------------------------------
+
+NormVariant norm_variant(uint32_t cols) {
+    if (cols < kNormVec) return kNormNarrow;
+    if (cols <= 512) return kNorm64x1;
+    if (cols <= 1024) return kNorm64x2;
+    if (cols <= 2048) return kNorm256x1;
+    if (cols <= 4096) return kNorm256x2;
+    if (cols <= 8192) return kNorm1024x1;
+    if (cols <= 16384) return kNorm1024x2;
+    return kNormLong;
+}
+
+uint32_t norm_lanes(NormVariant v) {
+    switch (v) {
+        case kNormNarrow: return 1;
+        case kNorm64x1:
+        case kNorm64x2: return 64;
+        case kNorm256x1:
+        case kNorm256x2: return 256;
+        default: return 1024;
+    }
+}
+
+struct Grid {
+    uint32_t grid, block;
+};
+
+Grid norm_grid(NormVariant v, uint32_t groups) {
+    const uint32_t lanes = norm_lanes(v), block = lanes < 256 ? 256 : lanes, each = block / lanes;
+    return {(groups + each - 1) / each, block};
+}
+
+// Row groups of a backward, per part: enough to fill the device, and each with as many rows as the others.
+uint32_t backward_groups(NormVariant v, uint32_t part_rows, uint32_t nparts) {
+    if (!part_rows) return 0;
+    uint32_t target = v == kNormNarrow ? 16384 : v == kNormLong ? 256 : norm_lanes(v) == 64 ? 4096 : norm_lanes(v) == 256 ? 1536 : 512;
+    target = std::max(1u, target / nparts);
+    const uint32_t each = (part_rows + target - 1) / target;
+    return (part_rows + each - 1) / each;
+}
+
+NormKernels kernels_for(int dtype, NormVariant v, bool stream32, bool q8) {
+    switch (dtype) {
+        case MEGRAY_FLOAT16: return norm_kernels_f16(v, stream32, q8);
+        case MRV_BFLOAT16: return norm_kernels_bf16(v, stream32, q8);
+        default: return norm_kernels_f32(v, stream32, q8);
+    }
+}
+
+Status launch_kernel(const void* kernel, dim3 grid, uint32_t block, const void* descriptor, hipStream_t stream) {
+    if (!grid.x) return MEGRAY_OK;
+    void* args[] = {const_cast<void*>(descriptor)};
+    HIP_CHECK(hipLaunchKernel(kernel, grid, dim3(block), args, 0, stream));
+    return MEGRAY_OK;
+}
+
+}  // namespace
+
+NormPlan::NormPlan() {
+    std::memset(&m_forward, 0, sizeof(m_forward));
+    std::memset(&m_backward, 0, sizeof(m_backward));
+    std::memset(&m_weight, 0, sizeof(m_weight));
+}
+
+void NormPlan::plan_forward(int collective, const mrv_rms_norm_call& c) {
+    const Shape s = check_shape(collective, c.nranks, c.rows, c.cols, c.dtype, c.residual_dtype, c.weight_dtype, c.eps);
+    const bool q8 = c.out_dtype == MEGRAY_INT8 || c.out_dtype == MRV_FLOAT8_E4M3;
+    if (!q8 && c.out_dtype != c.dtype) MEGRAY_THROW("the output's dtype is the sends', INT8 or FLOAT8_E4M3");
+    const size_t out_elem = q8 ? 1 : s.elem;
+    if (!c.sendbuffs) MEGRAY_THROW("sendbuffs is null");
+    if (!c.outs) MEGRAY_THROW("outs is null");
+    if (q8 && !c.scales) MEGRAY_THROW("an 8-bit output needs scales");
+    NormLaunch& L = m_forward;
+    L.send_stride = row_bytes(c.send_stride, s.cols, s.elem);
+    L.residual_stride = row_bytes(c.residual_stride, s.cols, s.stream_elem);
+    L.hidden_stride = row_bytes(c.residual_out_stride, s.cols, s.stream_elem);
+    L.out_stride = row_bytes(c.out_stride, s.cols, out_elem);
+    if (!s.rows) return;  // nothing to launch
+    std::vector<Rows> inputs, replaced, outputs;
+    std::vector<int> replaces;
+    auto input = [&](const void* p, uint64_t rows, uint64_t stride, size_t elem, uint64_t own_row) {
+        inputs.push_back({reinterpret_cast<uintptr_t>(p), rows, s.cols * elem, stride, uint32_t(elem)});
+        replaced.push_back(inputs.back());
+        replaced.back().at += own_row * stride;
+    };
+    auto output = [&](void* p, uint64_t stride, size_t elem, int replacing) {
+        outputs.push_back({reinterpret_cast<uintptr_t>(p), s.part_rows, s.cols * elem, stride, uint32_t(elem)});
+        replaces.push_back(replacing);
+    };
+    for (uint32_t r = 0; r < s.nranks; ++r) {
+        check_pointer(c.sendbuffs[r], s.elem, "a send buffer is null");
+        L.send[r] = c.sendbuffs[r];
+        input(c.sendbuffs[r], s.rows, L.send_stride, s.elem, s.gathered ? 0 : uint64_t(r) * s.part_rows);
+    }
+    const uint32_t residuals = c.residuals ? (s.gathered ? 1 : s.nranks) : 0;
+    for (uint32_t r = 0; r < residuals; ++r) {
+        check_pointer(c.residuals[r], s.stream_elem, "a residual is null");
+        L.residual[r] = c.residuals[r];
+        input(c.residuals[r], s.part_rows, L.residual_stride, s.stream_elem, 0);
+    }
+    check_pointer(c.weight, s.weight32 ? 4 : s.elem, "weight is null");
+    L.weight = c.weight;
+    inputs.push_back({reinterpret_cast<uintptr_t>(c.weight), 1, uint64_t(s.cols) * (s.weight32 ? 4 : s.elem), 0, 0});
+    replaced.push_back(inputs.back());
+    uint64_t written = 0;
+    for (uint32_t r = 0; r < s.nranks; ++r) {
+        check_pointer(c.outs[r], out_elem, "an output is null");
+        L.out[r] = c.outs[r];
+        output(c.outs[r], L.out_stride, out_elem, q8 ? -1 : int(r));
+        if (c.residual_outs) {
+            check_pointer(c.residual_outs[r], s.stream_elem, "a residual output is null");
+            L.hidden[r] = c.residual_outs[r];
+            output(c.residual_outs[r], L.hidden_stride, s.stream_elem, residuals ? int(s.nranks + (s.gathered ? 0 : r)) : -1);
+        }
+        if (q8) {
+            check_pointer(c.scales[r], 4, "a scale buffer is null");
+            L.scales[r] = c.scales[r];
+            outputs.push_back({reinterpret_cast<uintptr_t>(c.scales[r]), 1, uint64_t(s.part_rows) * 4, 0, 4});
+            replaces.push_back(-1);
+        }
+        written += uint64_t(s.part_rows) * s.cols * (out_elem + (c.residual_outs ? s.stream_elem : 0));
+    }
+    check_rows(outputs, replaces, inputs, replaced);
+    L.rows = s.rows;
+    L.part_rows = s.part_rows;
+    L.cols = s.cols;
+    L.nranks = s.nranks;
+    L.ndst = s.gathered ? s.nranks : 1;
+    L.weight32 = s.weight32;
+    L.int8 = c.out_dtype == MEGRAY_INT8;
+    L.keep = written <= kKeepMaxBytes;
+    L.has_hidden = c.residual_outs != nullptr;
+    L.eps = c.eps;
+    const NormVariant v = norm_variant(s.cols);
+    m_first = kernels_for(c.dtype, v, s.stream32, q8).forward;
+    const Grid g = norm_grid(v, s.rows);
+    m_grid = g.grid;
+    m_block = g.block;
+    m_descriptor = &m_forward;
+}
+
+size_t norm_backward_workspace(int collective, uint32_t nranks, size_t rows, size_t cols) {
+    check_collective(collective, nranks);
+    const uint32_t nparts = collective == MRV_ALL_REDUCE ? 1 : nranks;
+    if (rows >= (uint64_t(1) << 22)) MEGRAY_THROW("too many rows");
+    check_extent(uint64_t(rows) * nparts, cols);
+    return size_t(backward_groups(norm_variant(uint32_t(cols)), uint32_t(rows), nparts)) * nparts * cols * sizeof(float);
+}
+
+void NormPlan::plan_backward(int collective, const mrv_rms_norm_backward_call& c) {
+    const Shape s = check_shape(collective, c.nranks, c.rows, c.cols, c.dtype, c.residual_dtype, c.weight_dtype, c.eps);
+    if (!c.sendbuffs) MEGRAY_THROW("sendbuffs is null");
+    if (!c.hiddens) MEGRAY_THROW("hiddens is null");
+    if (!c.residual_out_grads && !c.send_grads && !c.weight_grads) MEGRAY_THROW("no gradient is asked for");
+    NormBackLaunch& L = m_backward;
+    L.send_stride = row_bytes(c.send_stride, s.cols, s.elem);
+    L.hidden_stride = row_bytes(c.hidden_stride, s.cols, s.stream_elem);
+    L.arriving_stride = row_bytes(c.residual_grad_stride, s.cols, s.stream_elem);
+    L.dhidden_stride = row_bytes(c.residual_out_grad_stride, s.cols, s.stream_elem);
+    L.dsend_stride = row_bytes(c.send_grad_stride, s.cols, s.elem);
+    std::vector<Rows> inputs, replaced, outputs;
+    std::vector<int> replaces;
+    const uint32_t copies = s.gathered ? 1 : s.nranks;
+    auto input = [&](const void* p, uint64_t rows, uint64_t stride, size_t elem, uint64_t own_row) {
+        inputs.push_back({reinterpret_cast<uintptr_t>(p), rows, s.cols * elem, stride, uint32_t(elem)});
+        replaced.push_back(inputs.back());
+        replaced.back().at += own_row * stride;
+    };
+    if (s.rows) {
+        for (uint32_t r = 0; r < s.nranks; ++r) {
+            check_pointer(c.sendbuffs[r], s.elem, "a send buffer is null");
+            L.send[r] = c.sendbuffs[r];
+            input(c.sendbuffs[r], s.rows, L.send_stride, s.elem, s.gathered ? 0 : uint64_t(r) * s.part_rows);
+        }
+        for (uint32_t r = 0; r < copies; ++r) {
+            check_pointer(c.hiddens[r], s.stream_elem, "a hidden state is null");
+            L.hidden[r] = c.hiddens[r];
+            input(c.hiddens[r], s.part_rows, L.hidden_stride, s.stream_elem, 0);
+        }
+        for (uint32_t r = 0; c.residual_grads && r < copies; ++r) {
+            check_pointer(c.residual_grads[r], s.stream_elem, "a residual gradient is null");
+            L.arriving[r] = c.residual_grads[r];
+            input(c.residual_grads[r], s.part_rows, L.arriving_stride, s.stream_elem, 0);
+        }
+        check_pointer(c.weight, s.weight32 ? 4 : s.elem, "weight is null");
+        L.weight = c.weight;
+        inputs.push_back({reinterpret_cast<uintptr_t>(c.weight), 1, uint64_t(s.cols) * (s.weight32 ? 4 : s.elem), 0, 0});
+        replaced.push_back(inputs.back());
+    }
+    const NormVariant v = norm_variant(s.cols);
+    const uint32_t nparts = s.gathered ? 1 : s.nranks;
+    const uint32_t part_groups = backward_groups(v, s.part_rows, nparts);
+    uint64_t written = 0;
+    for (uint32_t r = 0; r < s.nranks; ++r) {
+        const int own = int(s.gathered ? 0 : r);
+        if (c.residual_out_grads && s.rows) {
+            check_pointer(c.residual_out_grads[r], s.stream_elem, "a residual gradient output is null");
+            L.dhidden[r] = c.residual_out_grads[r];
+            outputs.push_back({reinterpret_cast<uintptr_t>(L.dhidden[r]), s.part_rows, s.cols * s.stream_elem, L.dhidden_stride, uint32_t(s.stream_elem)});
+            // in the hidden state's place, or in the arriving gradient's
+            const bool arriving = c.residual_grads && L.dhidden[r] == L.arriving[own];
+            replaces.push_back(int(s.nranks) + (arriving ? int(copies) : 0) + own);
+            written += uint64_t(s.part_rows) * s.cols * s.stream_elem;
+        }
+        if (c.send_grads && s.rows) {
+            check_pointer(c.send_grads[r], s.elem, "a send gradient is null");
+            L.dsend[r] = c.send_grads[r];
+            outputs.push_back({reinterpret_cast<uintptr_t>(L.dsend[r]), s.part_rows, s.cols * s.elem, L.dsend_stride, uint32_t(s.elem)});
+            replaces.push_back(int(r));
+            written += uint64_t(s.part_rows) * s.cols * s.elem;
+        }
+        if (c.weight_grads) {
+            check_pointer(c.weight_grads[r], 4, "a weight gradient is null");
+            m_weight.dweight[r] = c.weight_grads[r];
+            outputs.push_back({reinterpret_cast<uintptr_t>(c.weight_grads[r]), 1, uint64_t(s.cols) * 4, 0, 4});
+            replaces.push_back(-1);
+        }
+    }
+    if (c.weight_grads) {
+        const size_t need = size_t(part_groups) * nparts * s.cols * sizeof(float);
+        if (need) {
+            check_pointer(c.workspace, 4, "weight gradients need a workspace");
+            if (c.workspace_bytes < need) MEGRAY_THROW("the workspace is too small (see mrv_rms_norm_backward_workspace)");
+            outputs.push_back({reinterpret_cast<uintptr_t>(c.workspace), 1, need, 0, 4});
+            replaces.push_back(-1);
+        }
+        L.partial = static_cast<float*>(c.workspace);
+        m_weight.partial = L.partial;
+        m_weight.part_groups = part_groups;
+        m_weight.cols = s.cols;
+        m_weight.nparts = nparts;
+        m_weight.nranks = s.nranks;
+        m_second = norm_weight_kernel();
+    }
+    check_rows(outputs, replaces, inputs, replaced);
+    if (!s.rows) return;  // the weight gradients are zero then
+    L.rows = s.rows;
+    L.part_rows = s.part_rows;
+    L.part_groups = part_groups;
+    L.groups = part_groups * nparts;
+    L.cols = s.cols;
+    L.nranks = s.nranks;
+    L.ndst = s.gathered ? s.nranks : 1;
+    L.weight32 = s.weight32;
+    L.keep = written <= kKeepMaxBytes;
+    L.eps = c.eps;
+    m_first = kernels_for(c.dtype, v, s.stream32, false).backward;
+    const Grid g = norm_grid(v, L.groups);
+    m_grid = g.grid;
+    m_block = g.block;
+    m_descriptor = &m_backward;
+}
+
+Status NormPlan::launch(hipStream_t stream) const {
+    if (m_first) {
+        const Status st = launch_kernel(m_first, dim3(m_grid), m_block, m_descriptor, stream);
+        if (st != MEGRAY_OK) return st;
+    }
+    if (m_second)
+        return launch_kernel(m_second, dim3((m_weight.cols + 63) / 64, m_weight.nparts), kNormWeightThreads, &m_weight, stream);
+    return MEGRAY_OK;
+}
+
+// ---- AdamW ---------------------------------------------------------------------------------------
+
+namespace {
+
+struct Interval {
+    uintptr_t begin, end;
+    bool written;
+};
+
+// No output may overlap anything else.
+void check_intervals(std::vector<Interval>& all) {
+    std::sort(all.begin(), all.end(), [](const Interval& a, const Interval& b) { return a.begin < b.begin; });
+    uintptr_t end_any = 0, end_written = 0;
+    for (const Interval& x : all) {
+        if (x.begin < (x.written ? end_any : end_written)) MEGRAY_THROW("a tensor that is written overlaps another");
+        end_any = std::max(end_any, x.end);
+        if (x.written) end_written = std::max(end_written, x.end);
+    }
+}
+
+}  // namespace
+
+Adamw::Adamw(const mrv_adamw_tensors& t) {
+    if (t.grad_ranks < 1 || t.grad_ranks > kMaxRanks) MEGRAY_THROW("grad_ranks must be in [1, 32]");
+    const size_t grad_elem = float_size(t.grad_dtype, "unknown gradient dtype");
+    if (t.ntensors && (!t.lens || !t.grads)) MEGRAY_THROW("lens or grads is null");
+    m_can_step = t.params != nullptr;
+    size_t param_elem = 0;
+    bool state8 = false;
+    if (m_can_step) {
+        if (t.param_ranks < 1 || t.param_ranks > kMaxRanks) MEGRAY_THROW("param_ranks must be in [1, 32]");
+        param_elem = float_size(t.param_dtype, "unknown parameter dtype");
+        if (t.state_dtype != MEGRAY_FLOAT32 && t.state_dtype != MRV_FLOAT8_E4M3) MEGRAY_THROW("states are FLOAT32 or FLOAT8_E4M3");
+        state8 = t.state_dtype == MRV_FLOAT8_E4M3;
+        if (!t.masters && t.param_dtype != MEGRAY_FLOAT32) MEGRAY_THROW("masters is null and the parameters are not FLOAT32");
+        if (!t.exp_avgs || !t.exp_avg_sqs) MEGRAY_THROW("exp_avgs or exp_avg_sqs is null");
+        if (state8 && (!t.exp_avg_scales || !t.exp_avg_sq_scales)) MEGRAY_THROW("8-bit states need scales");
+    }
+    const uint32_t param_ranks = m_can_step ? t.param_ranks : 0;
+
+    uint64_t ntiles = 0;
+    for (size_t n = 0; n < t.ntensors; ++n) {
+        if (t.lens[n] > (uint64_t(1) << 40)) MEGRAY_THROW("a tensor is too long");
+        ntiles += (t.lens[n] + kAdamTile - 1) / kAdamTile;
+        // a grid counts its lanes in 32 bits
+        if (ntiles >= (uint64_t(1) << 24)) MEGRAY_THROW("too many elements for one handle");
+    }
+    if (t.ntensors >= (uint64_t(1) << 24)) MEGRAY_THROW("too many tensors for one handle");
+
+    // one table: tensors, tiles, gradient pointers, parameter pointers
+    const size_t tensors_bytes = t.ntensors * sizeof(AdamTensor), tiles_bytes = size_t(ntiles) * sizeof(AdamTile);
+    const size_t grads_bytes = t.ntensors * t.grad_ranks * sizeof(void*), params_bytes = t.ntensors * param_ranks * sizeof(void*);
+    std::vector<char> host(tensors_bytes + tiles_bytes + grads_bytes + params_bytes);
+    auto* tensors = reinterpret_cast<AdamTensor*>(host.data());
+    auto* tiles = reinterpret_cast<AdamTile*>(host.data() + tensors_bytes);
+    auto* grads = reinterpret_cast<const void**>(host.data() + tensors_bytes + tiles_bytes);
+    auto* params = reinterpret_cast<void**>(host.data() + tensors_bytes + tiles_bytes + grads_bytes);
+    std::vector<Interval> used;
+    auto take = [&](const void* p, uint64_t bytes, size_t align, bool written, const char* null_text) {
+        check_pointer(p, align, null_text);
+        const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+        used.push_back({a, a + bytes, written});
+    };
+    size_t tile = 0;
+    for (size_t n = 0; n < t.ntensors; ++n) {
+        const uint64_t len = t.lens[n];
+        AdamTensor& x = tensors[n];
+        std::memset(&x, 0, sizeof(x));
+        x.len = len;
+        if (!len) continue;
+        for (uint64_t k = 0; k * kAdamTile < len; ++k) tiles[tile++] = {uint32_t(n), uint32_t(k)};
+        for (uint32_t r = 0; r < t.grad_ranks; ++r) {
+            const void* p = t.grads[size_t(r) * t.ntensors + n];
+            take(p, len * grad_elem, grad_elem, false, "a gradient is null");
+            grads[n * t.grad_ranks + r] = p;
+        }
+        if (!m_can_step) continue;
+        for (uint32_t r = 0; r < param_ranks; ++r) {
+            void* p = t.params[size_t(r) * t.ntensors + n];
+            take(p, len * param_elem, param_elem, true, "a parameter is null");
+            params[n * param_ranks + r] = p;
+        }
+        x.master = t.masters ? t.masters[n] : static_cast<float*>(params[n * param_ranks]);
+        const bool shared = t.param_dtype == MEGRAY_FLOAT32 && x.master == params[n * param_ranks];
+        if (!shared) take(x.master, len * 4, 4, true, "a master is null");
+        const uint64_t blocks = (len + kAdamBlock - 1) / kAdamBlock;
+        x.m = t.exp_avgs[n];
+        x.v = t.exp_avg_sqs[n];
+        take(x.m, len * (state8 ? 1 : 4), state8 ? 1 : 4, true, "a running mean is null");
+        take(x.v, len * (state8 ? 1 : 4), state8 ? 1 : 4, true, "a running mean of squares is null");
+        if (state8) {
+            x.m_scale = t.exp_avg_scales[n];
+            x.v_scale = t.exp_avg_sq_scales[n];
+            take(x.m_scale, blocks * 4, 4, true, "a scale buffer is null");
+            take(x.v_scale, blocks * 4, 4, true, "a scale buffer is null");
+        }
+        x.decay = t.weight_decays ? t.weight_decays[n] : 0.0f;
+        if (!std::isfinite(x.decay)) MEGRAY_THROW("a weight decay is not finite");
+    }
+    check_intervals(used);
+
+    m_groups = uint32_t(std::min<uint64_t>(ntiles, kAdamNormGroups));
+    if (hipGetDevice(&m_device) != hipSuccess) {
+        (void)hipGetLastError();
+        throw HipFailure();
+    }
+    if (!host.empty()) {
+        if (hipMalloc(&m_table, host.size()) != hipSuccess) {
+            (void)hipGetLastError();
+            m_table = nullptr;
+            throw HipFailure();
+        }
+        if (hipMemcpy(m_table, host.data(), host.size(), hipMemcpyHostToDevice) != hipSuccess) {
+            (void)hipGetLastError();
+            (void)hipFree(m_table);
+            m_table = nullptr;
+            throw HipFailure();
+        }
+    }
+    const char* table = static_cast<const char*>(m_table);
+    m_norm.tensors = m_step.tensors = reinterpret_cast<const AdamTensor*>(table);
+    m_norm.tiles = m_step.tiles = reinterpret_cast<const AdamTile*>(table + tensors_bytes);
+    m_norm.grads = m_step.grads = reinterpret_cast<const void* const*>(table + tensors_bytes + tiles_bytes);
+    m_step.params = reinterpret_cast<void* const*>(const_cast<char*>(table) + tensors_bytes + tiles_bytes + grads_bytes);
+    m_norm.grad_ranks = m_step.grad_ranks = t.grad_ranks;
+    m_step.param_ranks = param_ranks;
+    m_norm.ntiles = m_step.ntiles = uint32_t(ntiles);
+    m_norm.groups = m_groups;
+    m_norm_kernel = adamw_norm_kernel_for(t.grad_dtype);
+    if (m_can_step) m_step_kernel = adamw_kernel_for(t.grad_dtype, t.param_dtype, state8);
+}
+
+Adamw::~Adamw() {
+    if (m_table) (void)hipFree(m_table);
+}
+
+void Adamw::check_device() const {
+    int device = -1;
+    if (hipGetDevice(&device) != hipSuccess) {
+        (void)hipGetLastError();
+        throw HipFailure();
+    }
+    if (device != m_device) MEGRAY_THROW("the handle's tables are on another device than the current one");
+}
+
+Status Adamw::grad_norm(float grad_scale, float max_norm, float* out, hipStream_t stream) const {
+    if (!out) MEGRAY_THROW("out is null");
+    if (reinterpret_cast<uintptr_t>(out) % 8) MEGRAY_THROW("out does not lie on a multiple of 8 bytes");
+    if (!std::isfinite(grad_scale)) MEGRAY_THROW("grad_scale is not finite");
+    if (!(max_norm >= 0.0f)) MEGRAY_THROW("max_norm must not be negative");
+    check_device();
+    AdamNormLaunch L = m_norm;
+    L.grad_scale = grad_scale;
+    L.max_norm = max_norm;
+    L.out = out;
+    const Status st = launch_kernel(m_norm_kernel, dim3(m_groups), kAdamThreads, &L, stream);
+    if (st != MEGRAY_OK) return st;
+    return launch_kernel(adamw_norm_join_kernel(), dim3(1), kAdamJoinThreads, &L, stream);
+}
+
+Status Adamw::step(const mrv_adamw_step_args& a, hipStream_t stream) const {
+    if (!m_can_step) MEGRAY_THROW("the handle was made without parameters: it has no step");
+    if (!std::isfinite(float(a.lr)) || !std::isfinite(float(a.grad_scale))) MEGRAY_THROW("lr or grad_scale is not finite");
+    if (!(a.beta1 >= 0 && a.beta1 < 1 && a.beta2 >= 0 && a.beta2 < 1)) MEGRAY_THROW("beta1 and beta2 must be in [0, 1)");
+    if (!(a.eps >= 0) || !std::isfinite(float(a.eps))) MEGRAY_THROW("eps must be finite and not negative");
+    if (a.step < 1) MEGRAY_THROW("step counts from 1");
+    if (reinterpret_cast<uintptr_t>(a.clip) % 4) MEGRAY_THROW("clip does not lie on a multiple of 4 bytes");
+    check_device();
+    AdamLaunch L = m_step;
+    L.lr = float(a.lr);
+    L.beta1 = float(a.beta1);
+    L.beta2 = float(a.beta2);
+    L.rest1 = float(1 - a.beta1);
+    L.rest2 = float(1 - a.beta2);
+    L.eps = float(a.eps);
+    L.rate = float(a.lr / (1 - std::pow(a.beta1, double(a.step))));
+    L.root_scale = float(1 / std::sqrt(1 - std::pow(a.beta2, double(a.step))));
+    L.grad_scale = float(a.grad_scale);
+    L.clip = a.clip;
+    return launch_kernel(m_step_kernel, dim3(L.ntiles), kAdamThreads, &L, stream);
+}
+
+}  // namespace vrank
+}  // namespace MegRay
