@@ -77,14 +77,15 @@ __device__ __forceinline__ u32x2 to_block(const float (&x)[8], float& scale) {
     float amax = __builtin_bit_cast(float, top);
     if (amax < kAmaxMin) amax = kAmaxMin;  // not true of a NaN
     const bool finite = amax < __builtin_inff();
-    const float inverse = kE4m3Max / amax;
-    scale = finite ? amax / kE4m3Max : __builtin_nanf("");
+    scale = amax / kE4m3Max;
+    const float inverse = 1.0f / scale;
     float q[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        q[i] = clamp_to(x[i] * inverse, kE4m3Max);
+        q[i] = clamp_to(quotient(x[i], scale, inverse), kE4m3Max);
         if (KeepAlive && x[i] > 0.0f) q[i] = __builtin_fmaxf(q[i], 0x1p-9f);
     }
+    if (!finite) scale = __builtin_nanf("");
     return finite ? to_e4m3(q) : u32x2{0x7f7f7f7fu, 0x7f7f7f7fu};
 }
 
@@ -132,8 +133,8 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const AdamLaunch L)
             v[j] *= v_scale;
             v[j] *= v[j];
         }
-        m[j] = __builtin_fmaf(L.rest1, x, L.beta1 * m[j]);
-        v[j] = __builtin_fmaf(L.rest2 * x, x, L.beta2 * v[j]);
+        m[j] = L.beta1 * m[j] + L.rest1 * x;
+        v[j] = L.beta2 * v[j] + L.rest2 * x * x;
         root[j] = __builtin_sqrtf(v[j]);
         const float update = L.rate * m[j] / __builtin_fmaf(root[j], L.root_scale, L.eps);
         p[j] = __builtin_fmaf(-shrink, p[j], p[j]) - update;

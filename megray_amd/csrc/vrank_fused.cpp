@@ -119,49 +119,67 @@ Shape check_shape(int collective, uint32_t nranks, size_t rows, size_t cols, int
 
 NormVariant norm_variant(uint32_t cols) {
     if (cols < kNormVec) return kNormNarrow;
-    if (cols <= 512) return kNorm64x1;
-    if (cols <= 1024) return kNorm64x2;
-    if (cols <= 2048) return kNorm256x1;
-    if (cols <= 4096) return kNorm256x2;
-    if (cols <= 8192) return kNorm1024x1;
-    if (cols <= 16384) return kNorm1024x2;
+    if (cols <= 64 * kNormVec) return kNormWave;
+    if (cols <= 1024 * kNormVec) return kNormBlock;
+    if (cols <= 2 * 1024 * kNormVec) return kNormBlock2;
     return kNormLong;
 }
 
-uint32_t norm_lanes(NormVariant v) {
+// Lanes of a workgroup, and the rows (forward) or row groups (backward) it takes.
+struct Layout {
+    uint32_t lanes, each;
+};
+
+Layout norm_layout(NormVariant v, uint32_t cols) {
+    const uint32_t per_lane = v == kNormBlock2 ? 2 * kNormVec : kNormVec;
     switch (v) {
-        case kNormNarrow: return 1;
-        case kNorm64x1:
-        case kNorm64x2: return 64;
-        case kNorm256x1:
-        case kNorm256x2: return 256;
-        default: return 1024;
+        case kNormNarrow: return {256, 256};
+        case kNormWave: return {256, 4};
+        case kNormLong: return {1024, 1};
+        default: return {(cols + 64 * per_lane - 1) / (64 * per_lane) * 64, 1};
     }
 }
 
-struct Grid {
-    uint32_t grid, block;
-};
+constexpr uint32_t kComputeUnits = 256;
 
-Grid norm_grid(NormVariant v, uint32_t groups) {
-    const uint32_t lanes = norm_lanes(v), block = lanes < 256 ? 256 : lanes, each = block / lanes;
-    return {(groups + each - 1) / each, block};
+// Workgroups that put sixteen wavefronts on every CU.
+uint32_t resident(uint32_t lanes) {
+    return kComputeUnits * std::max(1u, 1024 / lanes);
 }
 
-// Row groups of a backward, per part: enough to fill the device, and each with as many rows as the others.
-uint32_t backward_groups(NormVariant v, uint32_t part_rows, uint32_t nparts) {
+// Row groups of a backward, per part: enough to fill the device and no more than twice that, sixteen rows to each if there are (a group
+// writes its share of the weight's gradient once), as many to each as to the others.
+uint32_t backward_groups(NormVariant v, uint32_t cols, uint32_t part_rows, uint32_t nparts) {
     if (!part_rows) return 0;
-    uint32_t target = v == kNormNarrow ? 16384 : v == kNormLong ? 256 : norm_lanes(v) == 64 ? 4096 : norm_lanes(v) == 256 ? 1536 : 512;
+    const Layout layout = norm_layout(v, cols);
+    uint32_t target = v == kNormNarrow ? 16384 : v == kNormLong ? kComputeUnits : resident(layout.lanes) * layout.each;
     target = std::max(1u, target / nparts);
+    if (v != kNormNarrow) target = std::min(std::max(target, part_rows / 16), 2 * target);
     const uint32_t each = (part_rows + target - 1) / target;
     return (part_rows + each - 1) / each;
 }
 
-NormKernels kernels_for(int dtype, NormVariant v, bool stream32, bool q8) {
+constexpr uint64_t kLongBytes = uint64_t(256) << 20;  // written in all, from which a launch is a long one
+constexpr uint32_t kDealBytes = 256 << 10;  // of a buffer that an XCD writes in one run
+
+Deal deal_blocks(uint32_t blocks, uint64_t block_bytes) {
+    Deal d{0, 0};
+    while (d.shift < 6 && (block_bytes << (d.shift + 1)) <= kDealBytes) ++d.shift;
+    d.whole = blocks >> (d.shift + 3) << (d.shift + 3);
+    return d;
+}
+
+bool on_lines(const std::vector<Rows>& buffers) {
+    for (const Rows& b : buffers)
+        if (b.at % 128 || (b.rows > 1 && b.stride % 128)) return false;
+    return true;
+}
+
+NormKernels kernels_for(int dtype, NormVariant v, uint32_t nranks, bool stream32, bool lines, bool q8) {
     switch (dtype) {
-        case MEGRAY_FLOAT16: return norm_kernels_f16(v, stream32, q8);
-        case MRV_BFLOAT16: return norm_kernels_bf16(v, stream32, q8);
-        default: return norm_kernels_f32(v, stream32, q8);
+        case MEGRAY_FLOAT16: return (stream32 ? norm_kernels_f16_f32 : norm_kernels_f16)(v, nranks, lines, q8);
+        case MRV_BFLOAT16: return (stream32 ? norm_kernels_bf16_f32 : norm_kernels_bf16)(v, nranks, lines, q8);
+        default: return norm_kernels_f32(v, nranks, lines, q8);
     }
 }
 
@@ -194,15 +212,17 @@ void NormPlan::plan_forward(int collective, const mrv_rms_norm_call& c) {
     L.hidden_stride = row_bytes(c.residual_out_stride, s.cols, s.stream_elem);
     L.out_stride = row_bytes(c.out_stride, s.cols, out_elem);
     if (!s.rows) return;  // nothing to launch
-    std::vector<Rows> inputs, replaced, outputs;
+    std::vector<Rows> inputs, replaced, outputs, rows;
     std::vector<int> replaces;
-    auto input = [&](const void* p, uint64_t rows, uint64_t stride, size_t elem, uint64_t own_row) {
-        inputs.push_back({reinterpret_cast<uintptr_t>(p), rows, s.cols * elem, stride, uint32_t(elem)});
+    auto input = [&](const void* p, uint64_t count, uint64_t stride, size_t elem, uint64_t own_row) {
+        inputs.push_back({reinterpret_cast<uintptr_t>(p), count, s.cols * elem, stride, uint32_t(elem)});
+        rows.push_back(inputs.back());
         replaced.push_back(inputs.back());
         replaced.back().at += own_row * stride;
     };
     auto output = [&](void* p, uint64_t stride, size_t elem, int replacing) {
         outputs.push_back({reinterpret_cast<uintptr_t>(p), s.part_rows, s.cols * elem, stride, uint32_t(elem)});
+        rows.push_back(outputs.back());
         replaces.push_back(replacing);
     };
     for (uint32_t r = 0; r < s.nranks; ++r) {
@@ -250,10 +270,15 @@ void NormPlan::plan_forward(int collective, const mrv_rms_norm_call& c) {
     L.has_hidden = c.residual_outs != nullptr;
     L.eps = c.eps;
     const NormVariant v = norm_variant(s.cols);
-    m_first = kernels_for(c.dtype, v, s.stream32, q8).forward;
-    const Grid g = norm_grid(v, s.rows);
-    m_grid = g.grid;
-    m_block = g.block;
+    const Layout layout = norm_layout(v, s.cols);
+    m_first = kernels_for(c.dtype, v, s.nranks, s.stream32, on_lines(rows), q8).forward;
+    L.positions = (s.rows + layout.each - 1) / layout.each;
+    m_block = L.lanes = layout.lanes;
+    const bool long_launch = written >= kLongBytes;
+    const bool one_each = v == kNormNarrow || v == kNormLong || (long_launch && L.ndst > 4);
+    m_grid = one_each ? L.positions : std::min(L.positions, resident(layout.lanes));
+    L.deal = deal_blocks(L.positions, layout.each * L.send_stride);
+    L.pace.on = long_launch && L.ndst > 1;
     m_descriptor = &m_forward;
 }
 
@@ -262,7 +287,7 @@ size_t norm_backward_workspace(int collective, uint32_t nranks, size_t rows, siz
     const uint32_t nparts = collective == MRV_ALL_REDUCE ? 1 : nranks;
     if (rows >= (uint64_t(1) << 22)) MEGRAY_THROW("too many rows");
     check_extent(uint64_t(rows) * nparts, cols);
-    return size_t(backward_groups(norm_variant(uint32_t(cols)), uint32_t(rows), nparts)) * nparts * cols * sizeof(float);
+    return size_t(backward_groups(norm_variant(uint32_t(cols)), uint32_t(cols), uint32_t(rows), nparts)) * nparts * cols * sizeof(float);
 }
 
 void NormPlan::plan_backward(int collective, const mrv_rms_norm_backward_call& c) {
@@ -276,11 +301,12 @@ void NormPlan::plan_backward(int collective, const mrv_rms_norm_backward_call& c
     L.arriving_stride = row_bytes(c.residual_grad_stride, s.cols, s.stream_elem);
     L.dhidden_stride = row_bytes(c.residual_out_grad_stride, s.cols, s.stream_elem);
     L.dsend_stride = row_bytes(c.send_grad_stride, s.cols, s.elem);
-    std::vector<Rows> inputs, replaced, outputs;
+    std::vector<Rows> inputs, replaced, outputs, rows;
     std::vector<int> replaces;
     const uint32_t copies = s.gathered ? 1 : s.nranks;
-    auto input = [&](const void* p, uint64_t rows, uint64_t stride, size_t elem, uint64_t own_row) {
-        inputs.push_back({reinterpret_cast<uintptr_t>(p), rows, s.cols * elem, stride, uint32_t(elem)});
+    auto input = [&](const void* p, uint64_t count, uint64_t stride, size_t elem, uint64_t own_row) {
+        inputs.push_back({reinterpret_cast<uintptr_t>(p), count, s.cols * elem, stride, uint32_t(elem)});
+        rows.push_back(inputs.back());
         replaced.push_back(inputs.back());
         replaced.back().at += own_row * stride;
     };
@@ -307,7 +333,7 @@ void NormPlan::plan_backward(int collective, const mrv_rms_norm_backward_call& c
     }
     const NormVariant v = norm_variant(s.cols);
     const uint32_t nparts = s.gathered ? 1 : s.nranks;
-    const uint32_t part_groups = backward_groups(v, s.part_rows, nparts);
+    const uint32_t part_groups = backward_groups(v, s.cols, s.part_rows, nparts);
     uint64_t written = 0;
     for (uint32_t r = 0; r < s.nranks; ++r) {
         const int own = int(s.gathered ? 0 : r);
@@ -315,6 +341,7 @@ void NormPlan::plan_backward(int collective, const mrv_rms_norm_backward_call& c
             check_pointer(c.residual_out_grads[r], s.stream_elem, "a residual gradient output is null");
             L.dhidden[r] = c.residual_out_grads[r];
             outputs.push_back({reinterpret_cast<uintptr_t>(L.dhidden[r]), s.part_rows, s.cols * s.stream_elem, L.dhidden_stride, uint32_t(s.stream_elem)});
+            rows.push_back(outputs.back());
             // in the hidden state's place, or in the arriving gradient's
             const bool arriving = c.residual_grads && L.dhidden[r] == L.arriving[own];
             replaces.push_back(int(s.nranks) + (arriving ? int(copies) : 0) + own);
@@ -324,6 +351,7 @@ void NormPlan::plan_backward(int collective, const mrv_rms_norm_backward_call& c
             check_pointer(c.send_grads[r], s.elem, "a send gradient is null");
             L.dsend[r] = c.send_grads[r];
             outputs.push_back({reinterpret_cast<uintptr_t>(L.dsend[r]), s.part_rows, s.cols * s.elem, L.dsend_stride, uint32_t(s.elem)});
+            rows.push_back(outputs.back());
             replaces.push_back(int(r));
             written += uint64_t(s.part_rows) * s.cols * s.elem;
         }
@@ -362,10 +390,11 @@ void NormPlan::plan_backward(int collective, const mrv_rms_norm_backward_call& c
     L.weight32 = s.weight32;
     L.keep = written <= kKeepMaxBytes;
     L.eps = c.eps;
-    m_first = kernels_for(c.dtype, v, s.stream32, false).backward;
-    const Grid g = norm_grid(v, L.groups);
-    m_grid = g.grid;
-    m_block = g.block;
+    const Layout layout = norm_layout(v, s.cols);
+    m_first = kernels_for(c.dtype, v, s.nranks, s.stream32, on_lines(rows), false).backward;
+    m_grid = (L.groups + layout.each - 1) / layout.each;
+    m_block = L.lanes = layout.lanes;
+    L.deal = deal_blocks(v == kNormWave ? 0 : s.part_rows, L.send_stride);
     m_descriptor = &m_backward;
 }
 

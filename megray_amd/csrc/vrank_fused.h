@@ -25,7 +25,33 @@ namespace vrank {
 
 // ---- the norm behind a fold ------------------------------------------------------------------
 
+#ifdef __HIPCC__
+#define MRV_DEVICE __device__ __forceinline__
+#else
+#define MRV_DEVICE inline
+#endif
+
 constexpr uint32_t kNormVec = 8;             // elements a lane holds of a row at a time: 16 bytes of a 16-bit type
+
+// Which row a workgroup takes.  Workgroups go to the eight XCDs in turn; dealt out in runs of 2^shift, neighbouring rows are
+// written by one XCD, through one L2, at about the same time.  Positions from `whole` on keep their own row.
+struct Deal {
+    uint32_t shift, whole;
+    MRV_DEVICE uint32_t of(uint32_t n) const {
+        if (n >= whole) return n;
+        return (n >> (shift + 3) << (shift + 3)) + ((n & 7u) << shift) + ((n >> 3) & ((1u << shift) - 1u));
+    }
+};
+
+// Whether a wavefront's stores go one at a time.
+struct Pace {
+    uint32_t on;
+    MRV_DEVICE void wait() const {
+#ifdef __HIP_DEVICE_COMPILE__
+        if (on) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#endif
+    }
+};
 
 struct NormLaunch {
     const void* send[kMaxRanks];
@@ -45,6 +71,10 @@ struct NormLaunch {
     uint32_t keep;       // stores leave their data in the last-level cache
     uint32_t has_hidden;
     float eps;
+    uint32_t lanes;      // of a row, where a workgroup is one row: a multiple of 64
+    uint32_t positions;  // rows in units of what a workgroup takes at a time
+    Deal deal;           // of the positions
+    Pace pace;
 };
 
 struct NormBackLaunch {
@@ -66,6 +96,8 @@ struct NormBackLaunch {
     uint32_t weight32;
     uint32_t keep;
     float eps;
+    uint32_t lanes;
+    Deal deal;  // of a part's rows
 };
 
 struct NormWeightLaunch {  // the second launch of a backward: weight gradients from the row groups' sums
@@ -77,19 +109,22 @@ struct NormWeightLaunch {  // the second launch of a backward: weight gradients 
     uint32_t nranks;
 };
 
-// How a row is spread over lanes: kNorm<lanes>x<vectors per lane>; rows of fewer than eight elements have a lane each
-// (kNormNarrow), rows that no variant holds in registers are swept twice (kNormLong).
-enum NormVariant { kNormNarrow, kNorm64x1, kNorm64x2, kNorm256x1, kNorm256x2, kNorm1024x1, kNorm1024x2, kNormLong };
+// How a row is spread over lanes: rows of fewer than eight elements have a lane each (kNormNarrow), rows of up to 512
+// a wavefront (kNormWave), rows of up to 8192 and 16384 a workgroup of as many wavefronts as they fill with one and two vectors per lane
+// (kNormBlock, kNormBlock2), and longer ones are swept twice (kNormLong).
+enum NormVariant { kNormNarrow, kNormWave, kNormBlock, kNormBlock2, kNormLong };
 
 struct NormKernels {  // addresses usable with hipLaunchKernel; null where the type has no such form
     const void* forward;
     const void* backward;
 };
 
-// in vrank_norm_<type>.hip: sends of that type, a residual stream of it or of FLOAT32, an output of it or of 8 bits
-NormKernels norm_kernels_f16(NormVariant v, bool stream32, bool q8);
-NormKernels norm_kernels_bf16(NormVariant v, bool stream32, bool q8);
-NormKernels norm_kernels_f32(NormVariant v, bool stream32, bool q8);
+// in vrank_norm_<sends' type>[_<residual stream's type>].hip; `lines`: every row of every buffer begins on a cache line
+NormKernels norm_kernels_f16(NormVariant v, uint32_t nranks, bool lines, bool q8);
+NormKernels norm_kernels_f16_f32(NormVariant v, uint32_t nranks, bool lines, bool q8);
+NormKernels norm_kernels_bf16(NormVariant v, uint32_t nranks, bool lines, bool q8);
+NormKernels norm_kernels_bf16_f32(NormVariant v, uint32_t nranks, bool lines, bool q8);
+NormKernels norm_kernels_f32(NormVariant v, uint32_t nranks, bool lines, bool q8);
 constexpr uint32_t kNormWeightThreads = 1024;
 const void* norm_weight_kernel();  // grid: 64 columns each, parts
 

@@ -110,10 +110,41 @@ __device__ __forceinline__ void store8(char* p, const Raw8<T>& x, bool keep) {
     }
 }
 
+// Row stores.  Rows on cache lines go past the caches like the collectives' own results (or stay in the last-level cache:
+// `keep`); others leave lines that two wavefronts, or two rows, write a part of, and those are put together in the L2.
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+typedef int32_t i32x2 __attribute__((ext_vector_type(2)));
+constexpr int kStream = 18;  // sc1 | nt
+constexpr int kStay = 16;    // sc1
+template <typename T, bool Lines>
+__device__ __forceinline__ void store_row(char* row, uint32_t offset, const Raw8<T>& x, bool keep) {
+    if constexpr (Lines) {
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(row, 0, -1, 0x00020000);
+#pragma unroll
+        for (uint32_t i = 0; i < sizeof(T) / 2; ++i) {
+            if (keep) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, x.q[i]), rsrc, int(offset + 16 * i), 0, kStay);
+            else __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, x.q[i]), rsrc, int(offset + 16 * i), 0, kStream);
+        }
+    } else {
+        store8<T>(row + offset, x, true);
+    }
+}
+
 __device__ __forceinline__ void store_codes(char* p, u32x2 x, bool keep) {
     typedef Unaligned<1>::v2 V;
     if (keep) *as_global<V>(p) = x;
     else __builtin_nontemporal_store(x, as_global<V>(p));
+}
+
+template <bool Lines>
+__device__ __forceinline__ void store_row_codes(char* row, uint32_t offset, u32x2 x, bool keep) {
+    if constexpr (Lines) {
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(row, 0, -1, 0x00020000);
+        if (keep) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(i32x2, x), rsrc, int(offset), 0, kStay);
+        else __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(i32x2, x), rsrc, int(offset), 0, kStream);
+    } else {
+        store_codes(row + offset, x, true);
+    }
 }
 
 template <typename T>
@@ -154,6 +185,13 @@ constexpr float kAmaxMin = 0x1p-100f;  // what a scale is made from at least: Q 
 
 __device__ __forceinline__ float clamp_to(float x, float limit) {
     return __builtin_fmaxf(__builtin_fminf(x, limit), -limit);
+}
+
+// x / y, `inverse` = 1 / y: one correction of the product makes the quotient the rounded one (Markstein 1990), so that a code
+// is the one its definition says also where a product's last bit would move it across a border.
+__device__ __forceinline__ float quotient(float x, float y, float inverse) {
+    const float q = x * inverse;
+    return __builtin_fmaf(__builtin_fmaf(-q, y, x), inverse, q);
 }
 
 __device__ __forceinline__ u32x2 to_e4m3(const float (&f)[8]) {  // |f| <= 448

@@ -4,8 +4,8 @@
 namespace MegRay {
 namespace vrank {
 
-NormKernels norm_kernels_bf16(NormVariant v, bool stream32, bool q8) {
-    return detail::norm_kernels<__bf16>(v, stream32, q8);
+NormKernels norm_kernels_bf16(NormVariant v, uint32_t nranks, bool lines, bool q8) {
+    return detail::norm_kernels_for<__bf16, __bf16>(v, nranks, lines, q8);
 }
 
 }  // namespace vrank

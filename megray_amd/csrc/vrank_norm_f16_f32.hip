@@ -1,0 +1,12 @@
+// The norm behind a fold and its backward, partial activations of type FLOAT16, residual stream of FLOAT32.
+#include "vrank_norm_impl.hpp"
+
+namespace MegRay {
+namespace vrank {
+
+NormKernels norm_kernels_f16_f32(NormVariant v, uint32_t nranks, bool lines, bool q8) {
+    return detail::norm_kernels_for<_Float16, float>(v, nranks, lines, q8);
+}
+
+}  // namespace vrank
+}  // namespace MegRay

@@ -4,8 +4,8 @@
 namespace MegRay {
 namespace vrank {
 
-NormKernels norm_kernels_f32(NormVariant v, bool stream32, bool q8) {
-    return detail::norm_kernels<float>(v, stream32, q8);
+NormKernels norm_kernels_f32(NormVariant v, uint32_t nranks, bool lines, bool q8) {
+    return detail::norm_kernels_for<float, float>(v, nranks, lines, q8);
 }
 
 }  // namespace vrank
