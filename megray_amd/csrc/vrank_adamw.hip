@@ -2,9 +2,9 @@
 //
 // Both are one pass over the ranks' gradients, which are summed on the way: N reads of a gradient, and for the step one read
 // and one write of master, m and v and N writes of the parameter - 4 to 7 bytes per operation, HBM bound.  A workgroup
-// takes kAdamTile elements of one tensor (a table says which), a lane eight of them: 16 bytes per access of a
-// 16-bit type.  32 lanes hold the 256 elements that share the scale of an 8-bit state, so the block's maximum is a
-// reduction over half a wavefront and the new codes leave from the same registers.
+// takes kAdamTile elements of one tensor (a table says which); a wavefront takes 512 of them, a lane two pieces of four,
+// 256 apart (see Raw8).  So a piece of a wavefront is just the 256 elements that share the scale of an 8-bit state: their
+// maximum is one reduction across it, and the new codes leave from the same registers.
 #include "vrank_fused_impl.hpp"
 
 namespace MegRay {
@@ -14,19 +14,61 @@ namespace {
 
 using namespace fused;
 
-// The sum over ranks of `have` elements from element `i` on; `ptrs` are the tensor's buffers.
-template <typename G>
-__device__ __forceinline__ void fold_grads(const void* const* ptrs, uint32_t nranks, uint64_t i, uint32_t have, float (&g)[8]) {
+// The elements of a tensor that a lane works on.
+struct Elements {
+    uint64_t at[2];    // first element of each piece of four
+    uint32_t have[2];  // how many of the four are there
+    __device__ __forceinline__ Elements(uint32_t tile, uint64_t len) {
+        const uint64_t first = uint64_t(tile) * kAdamTile + threadIdx.x / 64 * 512u + threadIdx.x % 64 * 4u;
+#pragma unroll
+        for (uint32_t p = 0; p < 2; ++p) {
+            at[p] = first + p * kAdamBlock;
+            have[p] = at[p] >= len ? 0u : len - at[p] < 4 ? uint32_t(len - at[p]) : 4u;
+        }
+    }
+    __device__ __forceinline__ bool whole() const { return have[1] == 4; }
+    template <typename T, bool Once>
+    __device__ __forceinline__ Raw8<T> load(ConstBytes base) const {  // whole() lanes only
+        return load44<T, Once>(base + at[0] * sizeof(T), base + at[1] * sizeof(T));
+    }
+    template <typename T>
+    __device__ __forceinline__ void load_some(ConstBytes base, float (&f)[8]) const {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) f[i] = i % 4 < have[i / 4] ? load_one<T>(base + (at[i / 4] + i % 4) * sizeof(T)) : 0.0f;
+    }
+    // `Size` bytes per element; `tile_at`: the workgroup's first element
+    template <uint32_t Size, bool Lines>
+    __device__ __forceinline__ void store(Bytes base, uint64_t tile_at, const uint32_t* w) const {
+        if (whole()) {
+            const Bytes tile = base + tile_at * Size;  // the same for the whole wavefront
+#pragma unroll
+            for (uint32_t p = 0; p < 2; ++p) store_dwords<4 * Size, Lines, Size>(tile, uint32_t(at[p] - tile_at) * Size, w + p * Size, false);
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                if (i % 4 >= have[i / 4]) continue;
+                const Bytes q = base + (at[i / 4] + i % 4) * Size;
+                if constexpr (Size == 4) *(MRV_GLOBAL uint32_t*)q = w[i];
+                else if constexpr (Size == 2) *(MRV_GLOBAL uint16_t*)q = uint16_t(w[i / 2] >> (16 * (i % 2)));
+                else *(MRV_GLOBAL uint8_t*)q = uint8_t(w[i / 4] >> (8 * (i % 4)));
+            }
+        }
+    }
+};
+
+// The sum over ranks of a lane's elements; `ptrs` are the tensor's buffers.
+template <typename G, bool Once>
+__device__ __forceinline__ void fold_grads(const void* const* ptrs, uint32_t nranks, const Elements& e, float (&g)[8]) {
     constexpr uint32_t C = sizeof(G) == 4 ? 4 : 8;
 #pragma unroll
     for (int j = 0; j < 8; ++j) g[j] = 0.0f;
-    if (have == 8) {
+    if (e.whole()) {
         for (uint32_t r0 = 0; r0 < nranks; r0 += C) {
             const uint32_t left = nranks - r0;
             Raw8<G> x[C];
 #pragma unroll
-            for (uint32_t r = 0; r < C; ++r)  // past the last rank: its buffer again, not added
-                x[r] = load8<G, true>(static_cast<const char*>(ptrs[r0 + (r < left ? r : left - 1)]) + i * sizeof(G));
+            for (uint32_t r = 0; r < C; ++r)
+                if (r < left) x[r] = e.load<G, Once>(bytes_of(ptrs[r0 + r]));
 #pragma unroll
             for (uint32_t r = 0; r < C; ++r) {
                 if (r < left) {
@@ -37,56 +79,133 @@ __device__ __forceinline__ void fold_grads(const void* const* ptrs, uint32_t nra
                 }
             }
         }
-    } else if (have) {
+    } else if (e.have[0]) {
         for (uint32_t r = 0; r < nranks; ++r) {
             float f[8];
-            load_part<G>(static_cast<const char*>(ptrs[r]) + i * sizeof(G), have, f);
+            e.load_some<G>(bytes_of(ptrs[r]), f);
 #pragma unroll
             for (int j = 0; j < 8; ++j) g[j] += f[j];
         }
     }
 }
 
-__device__ __forceinline__ u32x2 load_codes(const char* p, uint32_t have) {
-    if (have == 8) return __builtin_nontemporal_load(as_global<Unaligned<1>::v2>(p));
-    u32x2 x = {0, 0};
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i)
-        if (i < have) x[i / 4] |= uint32_t(*as_global<uint8_t>(p + i)) << (8 * (i % 4));
-    return x;
-}
-
-__device__ __forceinline__ void store_codes_part(char* p, uint32_t have, u32x2 x) {
-    if (have == 8) {
-        store_codes(p, x, false);
-        return;
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i)
-        if (i < have) *as_global<uint8_t>(p + i) = uint8_t(x[i / 4] >> (8 * (i % 4)));
-}
-
-// Codes and scale of a block; all 32 lanes of it call this.  KeepAlive: a value above zero gets at least the smallest code, so that a
-// root of v that is small beside its block's largest does not vanish from the denominator.
+// Codes and scale of a block, four elements of it in each lane.  KeepAlive: a value above zero gets at least the smallest code, so
+// that a root of v that is small beside its block's largest does not vanish from the denominator.
 template <bool KeepAlive>
-__device__ __forceinline__ u32x2 to_block(const float (&x)[8], float& scale) {
+__device__ __forceinline__ uint32_t to_block(const float* x, float& scale) {
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = Larger()(top, magnitude(x[i]));
-    top = across_half(top, Larger());
-    float amax = __builtin_bit_cast(float, top);
+    for (int i = 0; i < 4; ++i) top = Larger()(top, magnitude(x[i]));
+    float amax = __builtin_bit_cast(float, across_wave(top, Larger()));
     if (amax < kAmaxMin) amax = kAmaxMin;  // not true of a NaN
     const bool finite = amax < __builtin_inff();
     scale = amax / kE4m3Max;
     const float inverse = 1.0f / scale;
-    float q[8];
+    float q[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
         q[i] = clamp_to(quotient(x[i], scale, inverse), kE4m3Max);
         if (KeepAlive && x[i] > 0.0f) q[i] = __builtin_fmaxf(q[i], 0x1p-9f);
     }
     if (!finite) scale = __builtin_nanf("");
-    return finite ? to_e4m3(q) : u32x2{0x7f7f7f7fu, 0x7f7f7f7fu};
+    return finite ? to_e4m3(q[0], q[1], q[2], q[3]) : 0x7f7f7f7fu;
+}
+
+// Lines: the tensor's buffers all begin on a cache line.
+template <typename G, typename P, bool State8, bool Lines>
+__device__ __forceinline__ void adamw_tile(const AdamLaunch& L, const AdamTensor& t, uint32_t tensor, uint32_t tile, float factor) {
+    const Elements e(tile, t.len);
+    const uint64_t tile_at = uint64_t(tile) * kAdamTile;
+    const uint64_t block = tile_at / kAdamBlock + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * 2;
+
+    float g[8], m[8], v[8], p[8];
+    uint32_t m_codes[2] = {0, 0}, v_codes[2] = {0, 0};
+    float m_scale[2] = {0.0f, 0.0f}, v_scale[2] = {0.0f, 0.0f};
+    if (e.whole()) {
+        Raw8<float> pr = e.load<float, Lines>(bytes_of(t.master)), mr, vr;
+        if constexpr (State8) {
+            typedef uint32_t V __attribute__((aligned(1)));
+#pragma unroll
+            for (uint32_t q = 0; q < 2; ++q) {
+                m_codes[q] = *(const MRV_GLOBAL V*)(bytes_of(t.m) + e.at[q]);
+                v_codes[q] = *(const MRV_GLOBAL V*)(bytes_of(t.v) + e.at[q]);
+            }
+        } else {
+            mr = e.load<float, Lines>(bytes_of(t.m));
+            vr = e.load<float, Lines>(bytes_of(t.v));
+        }
+        widen<float>(pr, p);
+        if constexpr (!State8) {
+            widen<float>(mr, m);
+            widen<float>(vr, v);
+        }
+    } else {
+        e.load_some<float>(bytes_of(t.master), p);
+        if constexpr (State8) {
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                if (i % 4 >= e.have[i / 4]) continue;
+                m_codes[i / 4] |= uint32_t(*(const MRV_GLOBAL uint8_t*)(bytes_of(t.m) + e.at[i / 4] + i % 4)) << (8 * (i % 4));
+                v_codes[i / 4] |= uint32_t(*(const MRV_GLOBAL uint8_t*)(bytes_of(t.v) + e.at[i / 4] + i % 4)) << (8 * (i % 4));
+            }
+        } else {
+            e.load_some<float>(bytes_of(t.m), m);
+            e.load_some<float>(bytes_of(t.v), v);
+        }
+    }
+    if constexpr (State8) {
+#pragma unroll
+        for (uint32_t q = 0; q < 2; ++q) {
+            if ((block + q) * kAdamBlock < t.len) {
+                m_scale[q] = load_one<float>(bytes_of(t.m_scale + block + q));
+                v_scale[q] = load_one<float>(bytes_of(t.v_scale + block + q));
+            }
+        }
+    }
+    fold_grads<G, Lines>(L.grads + uint64_t(tensor) * L.grad_ranks, L.grad_ranks, e, g);
+    if constexpr (State8) {
+        from_e4m3(u32x2{m_codes[0], m_codes[1]}, m);
+        from_e4m3(u32x2{v_codes[0], v_codes[1]}, v);
+    }
+    const float shrink = L.lr * t.decay;
+    float root[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float x = g[j] * factor;
+        if constexpr (State8) {
+            m[j] *= m_scale[j / 4];
+            v[j] *= v_scale[j / 4];
+            v[j] *= v[j];
+        }
+        m[j] = L.beta1 * m[j] + L.rest1 * x;
+        v[j] = L.beta2 * v[j] + L.rest2 * x * x;
+        root[j] = __builtin_sqrtf(v[j]);
+        const float update = L.rate * m[j] / __builtin_fmaf(root[j], L.root_scale, L.eps);
+        p[j] = __builtin_fmaf(-shrink, p[j], p[j]) - update;
+    }
+    e.store<4, Lines>(bytes_of(t.master), tile_at, narrow<float>(p).w);
+    const Raw8<P> param = narrow<P>(p);
+    for (uint32_t r = 0; r < L.param_ranks; ++r)
+        e.store<sizeof(P), Lines>(bytes_of(L.params[uint64_t(tensor) * L.param_ranks + r]), tile_at, param.w);
+    if constexpr (State8) {
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j)  // elements behind the tensor's end do not count for the block's maximum
+            if (j % 4 >= e.have[j / 4]) m[j] = root[j] = 0.0f;
+#pragma unroll
+        for (uint32_t q = 0; q < 2; ++q) {
+            m_codes[q] = to_block<false>(m + 4 * q, m_scale[q]);
+            v_codes[q] = to_block<true>(root + 4 * q, v_scale[q]);
+            if (threadIdx.x % 64 == 0 && (block + q) * kAdamBlock < t.len) {
+                store_one<float>(bytes_of(t.m_scale + block + q), m_scale[q]);
+                store_one<float>(bytes_of(t.v_scale + block + q), v_scale[q]);
+            }
+        }
+        e.store<1, Lines>(bytes_of(t.m), tile_at, m_codes);
+        e.store<1, Lines>(bytes_of(t.v), tile_at, v_codes);
+    } else {
+        e.store<4, Lines>(bytes_of(t.m), tile_at, narrow<float>(m).w);
+            e.store<4, Lines>(bytes_of(t.v), tile_at, narrow<float>(v).w);
+    }
 }
 
 template <typename G, typename P, bool State8>
@@ -97,73 +216,10 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const AdamLaunch L)
         if (!(__builtin_fabsf(clip) < __builtin_inff())) return;
         factor *= clip;
     }
-    const AdamTile where = L.tiles[blockIdx.x];
+    const AdamTile where = L.tiles[L.deal.of(blockIdx.x)];
     const AdamTensor t = L.tensors[where.tensor];
-    const uint64_t i = uint64_t(where.tile) * kAdamTile + threadIdx.x * kAdamVec;
-    const uint32_t have = i >= t.len ? 0u : t.len - i < kAdamVec ? uint32_t(t.len - i) : kAdamVec;
-    const uint64_t block = i / kAdamBlock;
-
-    float g[8], m[8], v[8], p[8];
-    float m_scale = 0.0f, v_scale = 0.0f;
-    u32x2 m_codes = {0, 0}, v_codes = {0, 0};
-    if constexpr (State8) {
-        if (have) {
-            m_codes = load_codes(static_cast<const char*>(t.m) + i, have);
-            v_codes = load_codes(static_cast<const char*>(t.v) + i, have);
-            m_scale = *as_global<float>(reinterpret_cast<const char*>(t.m_scale + block));
-            v_scale = *as_global<float>(reinterpret_cast<const char*>(t.v_scale + block));
-        }
-    } else {
-        load_part<float>(static_cast<const char*>(t.m) + i * 4, have, m);
-        load_part<float>(static_cast<const char*>(t.v) + i * 4, have, v);
-    }
-    load_part<float>(reinterpret_cast<const char*>(t.master + i), have, p);
-    fold_grads<G>(L.grads + uint64_t(where.tensor) * L.grad_ranks, L.grad_ranks, i, have, g);
-    if constexpr (State8) {
-        from_e4m3(m_codes, m);
-        from_e4m3(v_codes, v);
-    }
-    const float shrink = L.lr * t.decay;
-    float root[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float x = g[j] * factor;
-        if constexpr (State8) {
-            m[j] *= m_scale;
-            v[j] *= v_scale;
-            v[j] *= v[j];
-        }
-        m[j] = L.beta1 * m[j] + L.rest1 * x;
-        v[j] = L.beta2 * v[j] + L.rest2 * x * x;
-        root[j] = __builtin_sqrtf(v[j]);
-        const float update = L.rate * m[j] / __builtin_fmaf(root[j], L.root_scale, L.eps);
-        p[j] = __builtin_fmaf(-shrink, p[j], p[j]) - update;
-    }
-    store_part<float>(reinterpret_cast<char*>(t.master + i), have, p, false);
-    for (uint32_t r = 0; r < L.param_ranks; ++r) {
-        char* q = static_cast<char*>(L.params[uint64_t(where.tensor) * L.param_ranks + r]);
-        store_part<P>(q + i * sizeof(P), have, p, false);
-    }
-    if constexpr (State8) {
-        if (have < 8) {  // elements behind the tensor's end do not count for the block's maximum
-#pragma unroll
-            for (uint32_t j = 0; j < 8; ++j)
-                if (j >= have) m[j] = root[j] = 0.0f;
-        }
-        m_codes = to_block<false>(m, m_scale);
-        v_codes = to_block<true>(root, v_scale);
-        if (have) {
-            store_codes_part(static_cast<char*>(t.m) + i, have, m_codes);
-            store_codes_part(static_cast<char*>(t.v) + i, have, v_codes);
-            if (threadIdx.x % (kAdamBlock / kAdamVec) == 0) {
-                *as_global<float>(reinterpret_cast<char*>(t.m_scale + block)) = m_scale;
-                *as_global<float>(reinterpret_cast<char*>(t.v_scale + block)) = v_scale;
-            }
-        }
-    } else {
-        store_part<float>(static_cast<char*>(t.m) + i * 4, have, m, false);
-        store_part<float>(static_cast<char*>(t.v) + i * 4, have, v, false);
-    }
+    if (t.lines) adamw_tile<G, P, State8, true>(L, t, where.tensor, where.tile, factor);
+    else adamw_tile<G, P, State8, false>(L, t, where.tensor, where.tile, factor);
 }
 
 // Sum over a workgroup in a fixed order; the result is valid in lane 0.
@@ -184,12 +240,10 @@ template <typename G>
 __global__ void __launch_bounds__(kAdamThreads) adamw_norm_kernel(const AdamNormLaunch L) {
     double sum = 0.0;
     for (uint32_t n = blockIdx.x; n < L.ntiles; n += L.groups) {
-        const AdamTile where = L.tiles[n];
-        const uint64_t len = L.tensors[where.tensor].len;
-        const uint64_t i = uint64_t(where.tile) * kAdamTile + threadIdx.x * kAdamVec;
-        const uint32_t have = i >= len ? 0u : len - i < kAdamVec ? uint32_t(len - i) : kAdamVec;
+        const AdamTile where = L.tiles[L.deal.of(n)];
+        const Elements e(where.tile, L.tensors[where.tensor].len);
         float g[8];
-        fold_grads<G>(L.grads + uint64_t(where.tensor) * L.grad_ranks, L.grad_ranks, i, have, g);
+        fold_grads<G, true>(L.grads + uint64_t(where.tensor) * L.grad_ranks, L.grad_ranks, e, g);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const double x = double(g[j] * L.grad_scale);

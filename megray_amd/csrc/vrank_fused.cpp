@@ -51,18 +51,20 @@ bool same_place(const Rows& a, const Rows& b) {
     return a.at == b.at && a.elem == b.elem && (a.stride == b.stride || a.rows == 1);
 }
 
-// Every output against every input and output.  `replaces[o]` is the input that output o may be, or -1.
-void check_rows(const std::vector<Rows>& outputs, const std::vector<int>& replaces, const std::vector<Rows>& inputs,
+// Every output against every input and output.  `replaces[o]` is the input that output o may be, or -1.  Whether one is.
+bool check_rows(const std::vector<Rows>& outputs, const std::vector<int>& replaces, const std::vector<Rows>& inputs,
                 const std::vector<Rows>& replaced) {
+    bool in_place = false;
     for (size_t o = 0; o < outputs.size(); ++o) {
         for (size_t p = o + 1; p < outputs.size(); ++p)
             if (overlap(outputs[o], outputs[p])) MEGRAY_THROW("two outputs overlap");
         for (size_t i = 0; i < inputs.size(); ++i) {
             if (!overlap(outputs[o], inputs[i])) continue;
-            if (replaces[o] == int(i) && same_place(outputs[o], replaced[i])) continue;
-            MEGRAY_THROW("an output overlaps an input out of place");
+            if (replaces[o] != int(i) || !same_place(outputs[o], replaced[i])) MEGRAY_THROW("an output overlaps an input out of place");
+            in_place = true;
         }
     }
+    return in_place;
 }
 
 struct Shape {
@@ -142,17 +144,19 @@ Layout norm_layout(NormVariant v, uint32_t cols) {
 
 constexpr uint32_t kComputeUnits = 256;
 
-// Workgroups that put sixteen wavefronts on every CU.
-uint32_t resident(uint32_t lanes) {
-    return kComputeUnits * std::max(1u, 1024 / lanes);
+// Workgroups that the device holds at a time, by the registers of the kernels for so many ranks (norm_kernels_ranks in
+// vrank_norm_impl.hpp): a walk over rows with more of them than that would run its second half after its first.
+uint32_t resident(uint32_t lanes, uint32_t nranks, bool stream32, bool backward) {
+    const uint32_t waves = backward ? (nranks <= 2 ? 20 : 16) : nranks <= 2 ? 24 : nranks <= 4 && !stream32 ? 20 : 16;
+    return kComputeUnits * std::max(1u, waves * 64 / lanes);
 }
 
 // Row groups of a backward, per part: enough to fill the device and no more than twice that, sixteen rows to each if there are (a group
 // writes its share of the weight's gradient once), as many to each as to the others.
-uint32_t backward_groups(NormVariant v, uint32_t cols, uint32_t part_rows, uint32_t nparts) {
+uint32_t backward_groups(NormVariant v, uint32_t cols, uint32_t part_rows, uint32_t nranks, uint32_t nparts) {
     if (!part_rows) return 0;
     const Layout layout = norm_layout(v, cols);
-    uint32_t target = v == kNormNarrow ? 16384 : v == kNormLong ? kComputeUnits : resident(layout.lanes) * layout.each;
+    uint32_t target = v == kNormNarrow ? 16384 : v == kNormLong ? kComputeUnits : resident(layout.lanes, nranks, false, true) * layout.each;
     target = std::max(1u, target / nparts);
     if (v != kNormNarrow) target = std::min(std::max(target, part_rows / 16), 2 * target);
     const uint32_t each = (part_rows + target - 1) / target;
@@ -258,7 +262,7 @@ void NormPlan::plan_forward(int collective, const mrv_rms_norm_call& c) {
         }
         written += uint64_t(s.part_rows) * s.cols * (out_elem + (c.residual_outs ? s.stream_elem : 0));
     }
-    check_rows(outputs, replaces, inputs, replaced);
+    const bool in_place = check_rows(outputs, replaces, inputs, replaced);
     L.rows = s.rows;
     L.part_rows = s.part_rows;
     L.cols = s.cols;
@@ -276,7 +280,14 @@ void NormPlan::plan_forward(int collective, const mrv_rms_norm_call& c) {
     m_block = L.lanes = layout.lanes;
     const bool long_launch = written >= kLongBytes;
     const bool one_each = v == kNormNarrow || v == kNormLong || (long_launch && L.ndst > 4);
-    m_grid = one_each ? L.positions : std::min(L.positions, resident(layout.lanes));
+    m_grid = one_each ? L.positions : std::min(L.positions, resident(layout.lanes, s.nranks, s.stream32, false));
+    // Few rows: a CU would store a row to every destination while others idle (one row of 8192 to 8 ranks, hidden state and output:
+    // 256 KiB, 1.7 us at 64 bytes a clock).  Workgroups share the destinations instead, and read the row as often, from the caches.
+    // Not where a destination is an input: it would be read after it is written.
+    L.splits = 1;
+    if (v == kNormBlock && !in_place)
+        while (2 * L.splits <= L.ndst && 2 * L.splits * L.positions <= kComputeUnits) L.splits *= 2;
+    m_grid *= L.splits;
     L.deal = deal_blocks(L.positions, layout.each * L.send_stride);
     L.pace.on = long_launch && L.ndst > 1;
     m_descriptor = &m_forward;
@@ -287,7 +298,7 @@ size_t norm_backward_workspace(int collective, uint32_t nranks, size_t rows, siz
     const uint32_t nparts = collective == MRV_ALL_REDUCE ? 1 : nranks;
     if (rows >= (uint64_t(1) << 22)) MEGRAY_THROW("too many rows");
     check_extent(uint64_t(rows) * nparts, cols);
-    return size_t(backward_groups(norm_variant(uint32_t(cols)), uint32_t(cols), uint32_t(rows), nparts)) * nparts * cols * sizeof(float);
+    return size_t(backward_groups(norm_variant(uint32_t(cols)), uint32_t(cols), uint32_t(rows), nranks, nparts)) * nparts * cols * sizeof(float);
 }
 
 void NormPlan::plan_backward(int collective, const mrv_rms_norm_backward_call& c) {
@@ -333,7 +344,7 @@ void NormPlan::plan_backward(int collective, const mrv_rms_norm_backward_call& c
     }
     const NormVariant v = norm_variant(s.cols);
     const uint32_t nparts = s.gathered ? 1 : s.nranks;
-    const uint32_t part_groups = backward_groups(v, s.cols, s.part_rows, nparts);
+    const uint32_t part_groups = backward_groups(v, s.cols, s.part_rows, s.nranks, nparts);
     uint64_t written = 0;
     for (uint32_t r = 0; r < s.nranks; ++r) {
         const int own = int(s.gathered ? 0 : r);
@@ -466,10 +477,12 @@ Adamw::Adamw(const mrv_adamw_tensors& t) {
     auto* grads = reinterpret_cast<const void**>(host.data() + tensors_bytes + tiles_bytes);
     auto* params = reinterpret_cast<void**>(host.data() + tensors_bytes + tiles_bytes + grads_bytes);
     std::vector<Interval> used;
+    uintptr_t bits = 0;  // of the current tensor's buffers' addresses
     auto take = [&](const void* p, uint64_t bytes, size_t align, bool written, const char* null_text) {
         check_pointer(p, align, null_text);
         const uintptr_t a = reinterpret_cast<uintptr_t>(p);
         used.push_back({a, a + bytes, written});
+        bits |= a;
     };
     size_t tile = 0;
     for (size_t n = 0; n < t.ntensors; ++n) {
@@ -478,6 +491,7 @@ Adamw::Adamw(const mrv_adamw_tensors& t) {
         std::memset(&x, 0, sizeof(x));
         x.len = len;
         if (!len) continue;
+        bits = 0;
         for (uint64_t k = 0; k * kAdamTile < len; ++k) tiles[tile++] = {uint32_t(n), uint32_t(k)};
         for (uint32_t r = 0; r < t.grad_ranks; ++r) {
             const void* p = t.grads[size_t(r) * t.ntensors + n];
@@ -496,16 +510,17 @@ Adamw::Adamw(const mrv_adamw_tensors& t) {
         const uint64_t blocks = (len + kAdamBlock - 1) / kAdamBlock;
         x.m = t.exp_avgs[n];
         x.v = t.exp_avg_sqs[n];
+        x.decay = t.weight_decays ? t.weight_decays[n] : 0.0f;
+        if (!std::isfinite(x.decay)) MEGRAY_THROW("a weight decay is not finite");
         take(x.m, len * (state8 ? 1 : 4), state8 ? 1 : 4, true, "a running mean is null");
         take(x.v, len * (state8 ? 1 : 4), state8 ? 1 : 4, true, "a running mean of squares is null");
+        x.lines = bits % 128 == 0;  // the scales, a float per block, do not matter for it
         if (state8) {
             x.m_scale = t.exp_avg_scales[n];
             x.v_scale = t.exp_avg_sq_scales[n];
             take(x.m_scale, blocks * 4, 4, true, "a scale buffer is null");
             take(x.v_scale, blocks * 4, 4, true, "a scale buffer is null");
         }
-        x.decay = t.weight_decays ? t.weight_decays[n] : 0.0f;
-        if (!std::isfinite(x.decay)) MEGRAY_THROW("a weight decay is not finite");
     }
     check_intervals(used);
 
@@ -536,6 +551,7 @@ Adamw::Adamw(const mrv_adamw_tensors& t) {
     m_step.param_ranks = param_ranks;
     m_norm.ntiles = m_step.ntiles = uint32_t(ntiles);
     m_norm.groups = m_groups;
+    m_norm.deal = m_step.deal = deal_blocks(uint32_t(ntiles), uint64_t(kAdamTile) * grad_elem);
     m_norm_kernel = adamw_norm_kernel_for(t.grad_dtype);
     if (m_can_step) m_step_kernel = adamw_kernel_for(t.grad_dtype, t.param_dtype, state8);
 }

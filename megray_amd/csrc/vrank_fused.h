@@ -54,11 +54,11 @@ struct Pace {
 };
 
 struct NormLaunch {
-    const void* send[kMaxRanks];
-    void* out[kMaxRanks];
+    const void* send[kMaxRanks];  // the kernels read `send` and `hidden`, `out` and `scales` as one table each
     void* hidden[kMaxRanks];
-    const void* residual[kMaxRanks];  // all_reduce: entry 0; entry 0 null: no residual
+    void* out[kMaxRanks];
     float* scales[kMaxRanks];
+    const void* residual[kMaxRanks];  // all_reduce: entry 0; entry 0 null: no residual
     const void* weight;
     uint64_t send_stride, residual_stride, hidden_stride, out_stride;  // bytes from a row to the next
     uint32_t rows;       // of the fold: all of them
@@ -73,14 +73,15 @@ struct NormLaunch {
     float eps;
     uint32_t lanes;      // of a row, where a workgroup is one row: a multiple of 64
     uint32_t positions;  // rows in units of what a workgroup takes at a time
+    uint32_t splits;     // workgroups that share a row's destinations, each folding the row for itself
     Deal deal;           // of the positions
     Pace pace;
 };
 
 struct NormBackLaunch {
-    const void* send[kMaxRanks];         // partial gradients of y
+    const void* send[kMaxRanks];         // partial gradients of y; read with `dhidden` as one table
     void* dhidden[kMaxRanks];            // entry 0 null: not wanted
-    void* dsend[kMaxRanks];              // entry 0 null: not wanted
+    void* dsend[kMaxRanks];              // entry 0 null: not wanted; read with `hidden` as one table
     const void* hidden[kMaxRanks];       // all_reduce: entry 0
     const void* arriving[kMaxRanks];     // all_reduce: entry 0; null: none
     const void* weight;
@@ -133,8 +134,8 @@ const void* norm_weight_kernel();  // grid: 64 columns each, parts
 constexpr uint32_t kAdamThreads = 256;
 constexpr uint32_t kAdamVec = 8;                           // elements of a lane
 constexpr uint32_t kAdamTile = kAdamThreads * kAdamVec;    // elements of a workgroup
-constexpr uint32_t kAdamBlock = 256;                       // elements that share a scale of an 8-bit state: 32 lanes
-constexpr uint32_t kAdamNormGroups = 2048;                 // workgroups of the gradient norm, at most
+constexpr uint32_t kAdamBlock = 256;                       // elements that share a scale of an 8-bit state: half a wavefront's
+constexpr uint32_t kAdamNormGroups = 512;                  // workgroups of the gradient norm, at most
 
 struct AdamTensor {  // one per tensor, in device memory
     uint64_t len;
@@ -144,7 +145,7 @@ struct AdamTensor {  // one per tensor, in device memory
     float* m_scale;
     float* v_scale;
     float decay;
-    uint32_t reserved;
+    uint32_t lines;  // every buffer of the tensor begins on a cache line
 };
 
 struct AdamTile {
@@ -159,6 +160,7 @@ struct AdamLaunch {
     void* const* params;       // [tensor][rank]
     uint32_t grad_ranks, param_ranks;
     uint32_t ntiles;
+    Deal deal;  // of the tiles
     float lr, beta1, beta2, eps;
     float rest1, rest2;  // 1 - beta1, 1 - beta2, from 64 bits: a beta near 1 has few bits of them left
     float rate;        // lr / (1 - beta1^step)
@@ -174,9 +176,9 @@ struct AdamNormLaunch {
     uint32_t grad_ranks;
     uint32_t ntiles;
     uint32_t groups;
+    Deal deal;  // of the tiles
     float grad_scale;
     float max_norm;
-    uint32_t reserved;
     float* out;  // [0] the norm, [1] the coefficient, then `groups` 64-bit sums
 };
 

@@ -19,47 +19,89 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 template <int Align>
 struct Unaligned;
-template <>
-struct Unaligned<1> {
-    typedef u32x4 v4 __attribute__((aligned(1)));
-    typedef u32x2 v2 __attribute__((aligned(1)));
-};
-template <>
-struct Unaligned<2> {
-    typedef u32x4 v4 __attribute__((aligned(2)));
-};
-template <>
-struct Unaligned<4> {
-    typedef u32x4 v4 __attribute__((aligned(4)));
-};
+#define MRV_UNALIGNED(n)                             \
+    template <>                                      \
+    struct Unaligned<n> {                            \
+        typedef u32x4 v4 __attribute__((aligned(n))); \
+        typedef u32x2 v2 __attribute__((aligned(n))); \
+    };
+MRV_UNALIGNED(1)
+MRV_UNALIGNED(2)
+MRV_UNALIGNED(4)
+#undef MRV_UNALIGNED
 
 // Pointers out of a descriptor or a table are global memory; saying so keeps flat instructions out of the kernels.
 #define MRV_GLOBAL __attribute__((address_space(1)))
-template <typename V>
-__device__ __forceinline__ const MRV_GLOBAL V* as_global(const char* p) {
-    return (const MRV_GLOBAL V*)(uintptr_t)p;
+typedef MRV_GLOBAL char* Bytes;
+typedef const MRV_GLOBAL char* ConstBytes;
+__device__ __forceinline__ ConstBytes bytes_of(const void* p) {
+    return (ConstBytes)(uintptr_t)p;
 }
-template <typename V>
-__device__ __forceinline__ MRV_GLOBAL V* as_global(char* p) {
-    return (MRV_GLOBAL V*)(uintptr_t)p;
+__device__ __forceinline__ Bytes bytes_of(void* p) {
+    return (Bytes)(uintptr_t)p;
+}
+__device__ __forceinline__ Bytes bytes_of(float* p) {
+    return (Bytes)(uintptr_t)p;
 }
 
-// Eight elements of T as they lie in memory.
-template <typename T>
-struct Raw8 {
-    u32x4 q[sizeof(T) / 2];
+// Two pointer tables of a launch descriptor that lie behind each other, entry l in lane l: one access reads them, and they take two vector
+// registers where 64 entries would not fit the scalar ones.
+struct LaneTable {
+    uint32_t lo, hi;
+    __device__ __forceinline__ explicit LaneTable(size_t offset) {  // in the kernel's only argument
+        static_assert(2 * kMaxRanks == 64, "an entry per lane");
+        typedef const __attribute__((address_space(4))) char* Constant;
+        const Constant p = Constant(__builtin_amdgcn_kernarg_segment_ptr()) + offset + threadIdx.x % 64 * sizeof(void*);
+        lo = reinterpret_cast<const __attribute__((address_space(4))) uint32_t*>(p)[0];
+        hi = reinterpret_cast<const __attribute__((address_space(4))) uint32_t*>(p)[1];
+    }
+    __device__ __forceinline__ Bytes at(uint32_t entry) const {  // the same entry for the whole wavefront
+        const uint32_t a = __builtin_amdgcn_readlane(lo, entry), b = __builtin_amdgcn_readlane(hi, entry);
+        return (Bytes)(uint64_t(b) << 32 | a);
+    }
+    __device__ __forceinline__ Bytes first(uint32_t entry) const { return at(entry); }
+    __device__ __forceinline__ Bytes second(uint32_t entry) const { return at(kMaxRanks + entry); }
 };
 
-// `once`: the data is read by no one else soon, so it need not stay in the caches.
-template <typename T, bool Once>
-__device__ __forceinline__ Raw8<T> load8(const char* p) {
-    typedef typename Unaligned<sizeof(T)>::v4 V;
-    Raw8<T> x;
+// Eight elements of T as they lie in memory: one piece of eight, or two pieces of four.  A wavefront's accesses have to cover whole cache
+// lines one instruction at a time: eight 32-bit elements per lane are two 16-byte accesses 32 bytes apart, half of every line twice, which
+// past the caches (a store that streams) costs more than twice the time.  So wherever a 32-bit type takes part, the
+// lanes hold two pieces of four elements, the wavefront's second 256 elements behind its first: 16 bytes of a 32-bit type, 8 of a 16-bit one.
+template <typename T>
+struct Raw8 {
+    uint32_t w[2 * sizeof(T)];
+};
+
+template <uint32_t Count, bool Once, int Align>
+__device__ __forceinline__ void load_dwords(ConstBytes p, uint32_t* w) {
+    if constexpr (Count == 8) {
+        typedef typename Unaligned<Align>::v2 V;
+        const u32x2 x = Once ? __builtin_nontemporal_load((const MRV_GLOBAL V*)p) : *(const MRV_GLOBAL V*)p;
+        w[0] = x[0], w[1] = x[1];
+    } else {
+        typedef typename Unaligned<Align>::v4 V;
 #pragma unroll
-    for (uint32_t i = 0; i < sizeof(T) / 2; ++i) {
-        if constexpr (Once) x.q[i] = __builtin_nontemporal_load(as_global<V>(p) + i);
-        else x.q[i] = as_global<V>(p)[i];
+        for (uint32_t i = 0; i < Count / 16; ++i) {
+            const u32x4 x = Once ? __builtin_nontemporal_load((const MRV_GLOBAL V*)p + i) : ((const MRV_GLOBAL V*)p)[i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[4 * i + j] = x[j];
+        }
     }
+}
+
+// Eight consecutive elements.  `Once`: the data is read by no one else soon, so it need not stay in the caches.
+template <typename T, bool Once>
+__device__ __forceinline__ Raw8<T> load8(ConstBytes p) {
+    Raw8<T> x;
+    load_dwords<8 * sizeof(T), Once, sizeof(T)>(p, x.w);
+    return x;
+}
+// Two pieces of four.
+template <typename T, bool Once>
+__device__ __forceinline__ Raw8<T> load44(ConstBytes p, ConstBytes q) {
+    Raw8<T> x;
+    load_dwords<4 * sizeof(T), Once, sizeof(T)>(p, x.w);
+    load_dwords<4 * sizeof(T), Once, sizeof(T)>(q, x.w + sizeof(T));
     return x;
 }
 
@@ -67,17 +109,16 @@ template <typename T>
 __device__ __forceinline__ void widen(const Raw8<T>& x, float (&f)[8]) {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = __builtin_bit_cast(float, uint32_t(x.q[i / 4][i % 4]));
+        for (int i = 0; i < 8; ++i) f[i] = __builtin_bit_cast(float, x.w[i]);
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t w = x.q[0][i];
             if constexpr (__is_same(T, __bf16)) {
-                f[2 * i] = __builtin_bit_cast(float, w << 16);
-                f[2 * i + 1] = __builtin_bit_cast(float, w & 0xffff0000u);
+                f[2 * i] = __builtin_bit_cast(float, x.w[i] << 16);
+                f[2 * i + 1] = __builtin_bit_cast(float, x.w[i] & 0xffff0000u);
             } else {
-                f[2 * i] = float(__builtin_bit_cast(_Float16, uint16_t(w)));
-                f[2 * i + 1] = float(__builtin_bit_cast(_Float16, uint16_t(w >> 16)));
+                f[2 * i] = float(__builtin_bit_cast(_Float16, uint16_t(x.w[i])));
+                f[2 * i + 1] = float(__builtin_bit_cast(_Float16, uint16_t(x.w[i] >> 16)));
             }
         }
     }
@@ -88,88 +129,83 @@ __device__ __forceinline__ Raw8<T> narrow(const float (&f)[8]) {
     Raw8<T> x;
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x.q[i / 4][i % 4] = __builtin_bit_cast(uint32_t, f[i]);
+        for (int i = 0; i < 8; ++i) x.w[i] = __builtin_bit_cast(uint32_t, f[i]);
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             typedef T Pair __attribute__((ext_vector_type(2)));
             typedef float Wide __attribute__((ext_vector_type(2)));
-            x.q[0][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((Wide{f[2 * i], f[2 * i + 1]}), Pair));
+            x.w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((Wide{f[2 * i], f[2 * i + 1]}), Pair));
         }
     }
     return x;
 }
 
-template <typename T>
-__device__ __forceinline__ void store8(char* p, const Raw8<T>& x, bool keep) {
-    typedef typename Unaligned<sizeof(T)>::v4 V;
-#pragma unroll
-    for (uint32_t i = 0; i < sizeof(T) / 2; ++i) {
-        if (keep) as_global<V>(p)[i] = x.q[i];
-        else __builtin_nontemporal_store(x.q[i], as_global<V>(p) + i);
-    }
-}
-
-// Row stores.  Rows on cache lines go past the caches like the collectives' own results (or stay in the last-level cache:
+// Stores.  Rows on cache lines go past the caches like the collectives' own results (or stay in the last-level cache:
 // `keep`); others leave lines that two wavefronts, or two rows, write a part of, and those are put together in the L2.
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef int32_t i32x2 __attribute__((ext_vector_type(2)));
 constexpr int kStream = 18;  // sc1 | nt
 constexpr int kStay = 16;    // sc1
-template <typename T, bool Lines>
-__device__ __forceinline__ void store_row(char* row, uint32_t offset, const Raw8<T>& x, bool keep) {
-    if constexpr (Lines) {
-        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(row, 0, -1, 0x00020000);
-#pragma unroll
-        for (uint32_t i = 0; i < sizeof(T) / 2; ++i) {
-            if (keep) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, x.q[i]), rsrc, int(offset + 16 * i), 0, kStay);
-            else __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, x.q[i]), rsrc, int(offset + 16 * i), 0, kStream);
+template <uint32_t Count, bool Lines, int Align>
+__device__ __forceinline__ void store_dwords(Bytes base, uint32_t offset, const uint32_t* w, bool keep) {
+    if constexpr (Lines) {  // `base` is the same for the whole wavefront
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, -1, 0x00020000);
+        if constexpr (Count == 4) {
+            if (keep) __builtin_amdgcn_raw_buffer_store_b32(int32_t(w[0]), rsrc, int(offset), 0, kStay);
+            else __builtin_amdgcn_raw_buffer_store_b32(int32_t(w[0]), rsrc, int(offset), 0, kStream);
+        } else if constexpr (Count == 8) {
+            const i32x2 x = {int32_t(w[0]), int32_t(w[1])};
+            if (keep) __builtin_amdgcn_raw_buffer_store_b64(x, rsrc, int(offset), 0, kStay);
+            else __builtin_amdgcn_raw_buffer_store_b64(x, rsrc, int(offset), 0, kStream);
+        } else {
+            static_assert(Count == 16, "a piece of at most 16 bytes");
+            const i32x4 x = {int32_t(w[0]), int32_t(w[1]), int32_t(w[2]), int32_t(w[3])};
+            if (keep) __builtin_amdgcn_raw_buffer_store_b128(x, rsrc, int(offset), 0, kStay);
+            else __builtin_amdgcn_raw_buffer_store_b128(x, rsrc, int(offset), 0, kStream);
         }
+    } else if constexpr (Count == 4) {
+        typedef uint32_t V __attribute__((aligned(1)));
+        *(MRV_GLOBAL V*)(base + offset) = w[0];
+    } else if constexpr (Count == 8) {
+        typedef typename Unaligned<Align>::v2 V;
+        *(MRV_GLOBAL V*)(base + offset) = u32x2{w[0], w[1]};
     } else {
-        store8<T>(row + offset, x, true);
+        typedef typename Unaligned<Align>::v4 V;
+#pragma unroll
+        for (uint32_t i = 0; i < Count / 16; ++i)
+            ((MRV_GLOBAL V*)(base + offset))[i] = u32x4{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
     }
 }
-
-__device__ __forceinline__ void store_codes(char* p, u32x2 x, bool keep) {
-    typedef Unaligned<1>::v2 V;
-    if (keep) *as_global<V>(p) = x;
-    else __builtin_nontemporal_store(x, as_global<V>(p));
-}
-
-template <bool Lines>
-__device__ __forceinline__ void store_row_codes(char* row, uint32_t offset, u32x2 x, bool keep) {
-    if constexpr (Lines) {
-        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(row, 0, -1, 0x00020000);
-        if (keep) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(i32x2, x), rsrc, int(offset), 0, kStay);
-        else __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(i32x2, x), rsrc, int(offset), 0, kStream);
-    } else {
-        store_codes(row + offset, x, true);
-    }
+// Eight consecutive elements, through the caches.
+template <typename T>
+__device__ __forceinline__ void store8(Bytes p, const Raw8<T>& x) {
+    store_dwords<8 * sizeof(T), false, sizeof(T)>(p, 0, x.w, true);
 }
 
 template <typename T>
-__device__ __forceinline__ float load_one(const char* p) {
-    return float(*as_global<T>(p));
+__device__ __forceinline__ float load_one(ConstBytes p) {
+    return float(*(const MRV_GLOBAL T*)p);
 }
 template <typename T>
-__device__ __forceinline__ void store_one(char* p, float x) {
-    *as_global<T>(p) = T(x);
+__device__ __forceinline__ void store_one(Bytes p, float x) {
+    *(MRV_GLOBAL T*)p = T(x);
 }
 
 // The first `have` elements of eight, the others 0 / left alone.
 template <typename T>
-__device__ __forceinline__ void load_part(const char* p, uint32_t have, float (&f)[8]) {
+__device__ __forceinline__ void load_part(ConstBytes p, uint32_t have, float (&f)[8]) {
     if (have == 8u) {
-        widen<T>(load8<T, true>(p), f);
+        widen<T>(load8<T, false>(p), f);
     } else {
 #pragma unroll
         for (uint32_t i = 0; i < 8; ++i) f[i] = i < have ? load_one<T>(p + i * sizeof(T)) : 0.0f;
     }
 }
 template <typename T>
-__device__ __forceinline__ void store_part(char* p, uint32_t have, const float (&f)[8], bool keep) {
+__device__ __forceinline__ void store_part(Bytes p, uint32_t have, const float (&f)[8]) {
     if (have == 8u) {
-        store8<T>(p, narrow<T>(f), keep);
+        store8<T>(p, narrow<T>(f));
     } else {
 #pragma unroll
         for (uint32_t i = 0; i < 8; ++i)
@@ -194,15 +230,13 @@ __device__ __forceinline__ float quotient(float x, float y, float inverse) {
     return __builtin_fmaf(__builtin_fmaf(-q, y, x), inverse, q);
 }
 
-__device__ __forceinline__ u32x2 to_e4m3(const float (&f)[8]) {  // |f| <= 448
-    u32x2 r;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        int w = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i], f[4 * i + 1], 0, false);
-        w = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2], f[4 * i + 3], w, true);
-        r[i] = uint32_t(w);
-    }
-    return r;
+__device__ __forceinline__ uint32_t to_e4m3(float a, float b, float c, float d) {  // at most 448 in magnitude
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+    return uint32_t(w);
+}
+__device__ __forceinline__ u32x2 to_e4m3(const float (&f)[8]) {
+    return {to_e4m3(f[0], f[1], f[2], f[3]), to_e4m3(f[4], f[5], f[6], f[7])};
 }
 
 __device__ __forceinline__ void from_e4m3(u32x2 x, float (&f)[8]) {

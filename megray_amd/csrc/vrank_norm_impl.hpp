@@ -54,33 +54,54 @@ struct RowReduce {
     }
 };
 
-// Which elements of a row a lane holds.
-template <uint32_t Vecs>
+// Which elements of a row a lane holds: `Vecs` times one piece of eight, or two of four (Split: where a 32-bit type takes part, see Raw8).
+// A piece that would pass the row's end is moved back to end with it.
+template <uint32_t Vecs, bool Split>
 struct RowPart {
-    uint32_t col[Vecs];     // first element of vector k, never past cols - 8
-    uint32_t repeat[Vecs];  // leading elements that belong to another lane (8 and more: all of them)
+    static constexpr uint32_t kPieces = Split ? 2 : 1, kWidth = kNormVec / kPieces;
+    uint32_t col[Vecs][kPieces];     // first element, never past cols - kWidth
+    uint32_t repeat[Vecs][kPieces];  // leading elements that belong to another lane (kWidth and more: all of them)
     __device__ __forceinline__ RowPart(uint32_t cols, uint32_t lanes, uint32_t lane) {
 #pragma unroll
         for (uint32_t k = 0; k < Vecs; ++k) {
-            const uint32_t want = (k * lanes + lane) * kNormVec;
-            col[k] = want + kNormVec <= cols ? want : cols - kNormVec;
-            repeat[k] = want - col[k];
+#pragma unroll
+            for (uint32_t p = 0; p < kPieces; ++p) {
+                const uint32_t first = Split ? (lane / 64 * 2 + p) * 64 + lane % 64 : lane;
+                const uint32_t want = k * lanes * kNormVec + first * kWidth;
+                col[k][p] = want + kWidth <= cols ? want : cols - kWidth;
+                repeat[k][p] = want - col[k][p];
+            }
         }
     }
-    __device__ __forceinline__ bool stores(uint32_t k) const { return repeat[k] < kNormVec; }
+    __device__ __forceinline__ bool mine(uint32_t k, uint32_t element) const {
+        return element % kWidth >= repeat[k][element / kWidth];
+    }
+    // element vector k of the row at `row`
+    template <typename T, bool Once>
+    __device__ __forceinline__ Raw8<T> load(ConstBytes row, uint32_t k) const {
+        if constexpr (Split) return load44<T, Once>(row + col[k][0] * uint32_t(sizeof(T)), row + col[k][kPieces - 1] * uint32_t(sizeof(T)));
+        else return load8<T, Once>(row + col[k][0] * uint32_t(sizeof(T)));
+    }
+    // `w`: the vector's eight elements, `Size` bytes each
+    template <uint32_t Size, bool Lines>
+    __device__ __forceinline__ void store(Bytes row, uint32_t k, const uint32_t* w, bool keep) const {
+#pragma unroll
+        for (uint32_t p = 0; p < kPieces; ++p)
+            if (repeat[k][p] < kWidth) store_dwords<kWidth * Size, Lines, Size>(row, col[k][p] * Size, w + p * kWidth * Size / 4, keep);
+    }
 };
 
 // Adds a row of `Ranks` consecutive ranks to `acc`, all loads issued before the first sum.  Not Whole: `left` of them are
 // there, and the last one's loads are repeated, not added.
-template <typename T, bool Lines, uint32_t Vecs, uint32_t Ranks, bool Whole>
-__device__ __forceinline__ void fold_ranks(const void* const* send, uint64_t row_offset, uint32_t left,
-                                           const uint32_t (&col)[Vecs], float (&acc)[Vecs][8]) {
+template <typename T, bool Lines, uint32_t Vecs, uint32_t Ranks, bool Whole, typename Part>
+__device__ __forceinline__ void fold_ranks(const LaneTable& table, uint32_t from, uint64_t row_offset, uint32_t left, const Part& part,
+                                           float (&acc)[Vecs][8]) {
     Raw8<T> x[Ranks][Vecs];
 #pragma unroll
     for (uint32_t r = 0; r < Ranks; ++r) {
-        const char* p = static_cast<const char*>(send[Whole || r < left ? r : left - 1]) + row_offset;
+        const ConstBytes p = table.first(from + (Whole || r < left ? r : left - 1)) + row_offset;
 #pragma unroll
-        for (uint32_t k = 0; k < Vecs; ++k) x[r][k] = load8<T, Lines>(p + col[k] * uint32_t(sizeof(T)));
+        for (uint32_t k = 0; k < Vecs; ++k) x[r][k] = part.template load<T, Lines>(p, k);
     }
 #pragma unroll
     for (uint32_t r = 0; r < Ranks; ++r) {
@@ -100,16 +121,18 @@ __device__ __forceinline__ void fold_ranks(const void* const* send, uint64_t row
 template <typename T, bool Lines, uint32_t Vecs, uint32_t Ranks>
 struct FirstRanks {
     Raw8<T> x[Ranks][Vecs];
-    __device__ __forceinline__ void load(const void* const* send, uint32_t nranks, uint64_t row_offset, const uint32_t (&col)[Vecs]) {
+    template <typename Part>
+    __device__ __forceinline__ void load(const LaneTable& table, uint32_t nranks, uint64_t row_offset, const Part& part) {
 #pragma unroll
         for (uint32_t r = 0; r < Ranks; ++r) {  // past the last rank: its buffer again, not added
-            const char* p = static_cast<const char*>(send[r < nranks ? r : nranks - 1]) + row_offset;
+            const ConstBytes p = table.first(r < nranks ? r : nranks - 1) + row_offset;
 #pragma unroll
-            for (uint32_t k = 0; k < Vecs; ++k) x[r][k] = load8<T, Lines>(p + col[k] * uint32_t(sizeof(T)));
+            for (uint32_t k = 0; k < Vecs; ++k) x[r][k] = part.template load<T, Lines>(p, k);
         }
     }
     // Adds them and the row's other ranks up.
-    __device__ __forceinline__ void fold(const void* const* send, uint32_t nranks, uint64_t row_offset, const uint32_t (&col)[Vecs],
+    template <typename Part>
+    __device__ __forceinline__ void fold(const LaneTable& table, uint32_t nranks, uint64_t row_offset, const Part& part,
                                          float (&acc)[Vecs][8]) const {
 #pragma unroll
         for (uint32_t k = 0; k < Vecs; ++k)
@@ -128,27 +151,24 @@ struct FirstRanks {
             }
         }
         uint32_t r = Ranks;
-        for (; r + Ranks <= nranks; r += Ranks) fold_ranks<T, Lines, Vecs, Ranks, true>(send + r, row_offset, Ranks, col, acc);
-        if (r < nranks) fold_ranks<T, Lines, Vecs, Ranks, false>(send + r, row_offset, nranks - r, col, acc);
+        for (; r + Ranks <= nranks; r += Ranks) fold_ranks<T, Lines, Vecs, Ranks, true>(table, r, row_offset, Ranks, part, acc);
+        if (r < nranks) fold_ranks<T, Lines, Vecs, Ranks, false>(table, r, row_offset, nranks - r, part, acc);
     }
 };
 
-template <typename T, uint32_t Vecs>
-__device__ __forceinline__ void load_weight(const void* weight, uint32_t weight32, const uint32_t (&col)[Vecs], float (&w)[Vecs][8]) {
-#pragma unroll
-    for (uint32_t k = 0; k < Vecs; ++k) {
-        if (weight32) widen<float>(load8<float, false>(static_cast<const char*>(weight) + uint64_t(col[k]) * 4), w[k]);
-        else widen<T>(load8<T, false>(static_cast<const char*>(weight) + uint64_t(col[k]) * sizeof(T)), w[k]);
-    }
+template <typename T, typename Part>
+__device__ __forceinline__ void load_weight(const void* weight, uint32_t weight32, const Part& part, uint32_t k, float (&w)[8]) {
+    if (weight32) widen<float>(part.template load<float, false>(bytes_of(weight), k), w);
+    else widen<T>(part.template load<T, false>(bytes_of(weight), k), w);
 }
 
 // A row of `ptr` (null: zeros), as it lies in memory.
-template <typename R, bool Lines, uint32_t Vecs>
-__device__ __forceinline__ void load_row(const void* ptr, uint64_t row_offset, const uint32_t (&col)[Vecs], Raw8<R> (&x)[Vecs]) {
+template <typename R, bool Lines, uint32_t Vecs, typename Part>
+__device__ __forceinline__ void load_row(ConstBytes ptr, uint64_t row_offset, const Part& part, Raw8<R> (&x)[Vecs]) {
     if (ptr) {
-        const char* p = static_cast<const char*>(ptr) + row_offset;
+        const ConstBytes p = ptr + row_offset;
 #pragma unroll
-        for (uint32_t k = 0; k < Vecs; ++k) x[k] = load8<R, Lines>(p + col[k] * uint32_t(sizeof(R)));
+        for (uint32_t k = 0; k < Vecs; ++k) x[k] = part.template load<R, Lines>(p, k);
     } else {
 #pragma unroll
         for (uint32_t k = 0; k < Vecs; ++k) x[k] = Raw8<R>{};
@@ -169,14 +189,16 @@ __device__ __forceinline__ bool row_scale(float r, uint32_t top, uint32_t int8, 
 // R: the residual stream's type.  Q8: 8-bit output with a scale per row.  Wave: a row is one wavefront's.  Lines: every row of every
 // buffer begins on a cache line.
 template <typename T, typename R, bool Q8, uint32_t Vecs, bool Wave, bool Lines, uint32_t Ranks>
-__global__ void __launch_bounds__(Wave ? 64 * kWaveRows : 1024) rms_norm_kernel(const NormLaunch L) {
+__global__ void __launch_bounds__(Wave ? 64 * kWaveRows : 1024, 4) rms_norm_kernel(const NormLaunch L) {
     typedef RowReduce<Wave, 1, Q8> Reduce;
     __shared__ typename Reduce::Shared shared;
     const uint32_t lanes = Wave ? 64 : L.lanes, lane = Wave ? threadIdx.x % 64 : threadIdx.x;
     const uint32_t wave_row = Wave ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : 0;
-    const RowPart<Vecs> part(L.cols, lanes, lane);
+    const LaneTable sends(offsetof(NormLaunch, send)), results(offsetof(NormLaunch, out));  // and hidden states; and scales
+    const RowPart<Vecs, sizeof(T) == 4 || sizeof(R) == 4> part(L.cols, lanes, lane);
     float w[Vecs][8];
-    load_weight<T, Vecs>(L.weight, L.weight32, part.col, w);
+#pragma unroll
+    for (uint32_t k = 0; k < Vecs; ++k) load_weight<T>(L.weight, L.weight32, part, k, w[k]);
 
     // The next row's loads are issued before this one's stores: a workgroup that only stored would leave its share of the
     // reads idle.  Two vectors per lane leave no registers for that.
@@ -191,16 +213,19 @@ __global__ void __launch_bounds__(Wave ? 64 * kWaveRows : 1024) rms_norm_kernel(
         return position < L.positions && row < L.rows;
     };
     auto fetch = [&] {
-        load_row<R, Lines, Vecs>(L.residual[0] ? L.residual[first] : nullptr, uint64_t(at) * L.residual_stride, part.col, residual);
-        ahead.load(L.send, L.nranks, uint64_t(row) * L.send_stride, part.col);
+        load_row<R, Lines, Vecs>(bytes_of(L.residual[0] ? L.residual[first] : nullptr), uint64_t(at) * L.residual_stride, part, residual);
+        ahead.load(sends, L.nranks, uint64_t(row) * L.send_stride, part);
     };
-    bool there = find(blockIdx.x);
+    // destinations of this workgroup
+    const uint32_t split = Wave || L.splits == 1 ? 0 : blockIdx.x % L.splits, start = Wave || L.splits == 1 ? blockIdx.x : blockIdx.x / L.splits;
+    const uint32_t dst = L.ndst * split / L.splits, dst_end = L.ndst * (split + 1) / L.splits;
+    bool there = find(start);
     if (kAhead && there) fetch();
     uint32_t slot = 0;
-    for (uint32_t position = blockIdx.x; there; slot ^= 1) {
+    for (uint32_t position = start; there; slot ^= 1) {
         float h[Vecs][8];
         if (!kAhead) fetch();
-        ahead.fold(L.send, L.nranks, uint64_t(row) * L.send_stride, part.col, h);
+        ahead.fold(sends, L.nranks, uint64_t(row) * L.send_stride, part, h);
         float sum[1] = {0.0f};
         uint32_t top = 0;
 #pragma unroll
@@ -210,12 +235,12 @@ __global__ void __launch_bounds__(Wave ? 64 * kWaveRows : 1024) rms_norm_kernel(
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 h[k][i] += f[i];
-                sum[0] = __builtin_fmaf(h[k][i], uint32_t(i) >= part.repeat[k] ? h[k][i] : 0.0f, sum[0]);
+                sum[0] = __builtin_fmaf(h[k][i], part.mine(k, uint32_t(i)) ? h[k][i] : 0.0f, sum[0]);
                 if (Q8) top = Larger()(top, magnitude(h[k][i] * w[k][i]));
             }
         }
         const uint32_t to = first, to_row = at;
-        position += gridDim.x;
+        position += gridDim.x;  // a launch with split rows has a workgroup for each
         there = find(position);
         if (kAhead && there) fetch();
         Reduce::run(shared, lanes / 64, slot, sum, top);
@@ -225,37 +250,33 @@ __global__ void __launch_bounds__(Wave ? 64 * kWaveRows : 1024) rms_norm_kernel(
         bool finite = true;
         if (Q8) {
             finite = row_scale(r, top, L.int8, scale, inverse);
-            if (lane == 0)
-                for (uint32_t d = 0; d < L.ndst; ++d) *as_global<float>(reinterpret_cast<char*>(L.scales[to + d] + to_row)) = scale;
+            for (uint32_t d = dst; d < dst_end; ++d)
+                if (lane == 0) *(MRV_GLOBAL float*)(results.second(to + d) + uint64_t(to_row) * 4) = scale;
         }
         const uint64_t hidden_row = uint64_t(to_row) * L.hidden_stride, out_row = uint64_t(to_row) * L.out_stride;
 #pragma unroll
         for (uint32_t k = 0; k < Vecs; ++k) {
-            if (!part.stores(k)) continue;
             const Raw8<R> stored = narrow<R>(h[k]);
             float y[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] = h[k][i] * r * w[k][i];
-            u32x2 codes = {0, 0};
             Raw8<T> result;
             if constexpr (Q8) {
                 const float limit = L.int8 ? kInt8Max : kE4m3Max;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] = clamp_to(quotient(y[i], scale, inverse), limit);
-                codes = L.int8 ? to_int8(y) : to_e4m3(y);
+                u32x2 codes = L.int8 ? to_int8(y) : to_e4m3(y);
                 if (!finite) codes = L.int8 ? u32x2{0, 0} : u32x2{0x7f7f7f7fu, 0x7f7f7f7fu};
+                result.w[0] = codes[0], result.w[1] = codes[1];
             } else {
                 result = narrow<T>(y);
             }
-            for (uint32_t d = 0; d < L.ndst; ++d) {
+            for (uint32_t d = dst; d < dst_end; ++d) {
                 if (L.has_hidden) {
-                    store_row<R, Lines>(static_cast<char*>(L.hidden[to + d]) + hidden_row, part.col[k] * uint32_t(sizeof(R)), stored, L.keep);
+                    part.template store<sizeof(R), Lines>(sends.second(to + d) + hidden_row, k, stored.w, L.keep);
                     L.pace.wait();
                 }
-                if constexpr (Q8)
-                    store_row_codes<Lines>(static_cast<char*>(L.out[to + d]) + out_row, part.col[k], codes, L.keep);
-                else
-                    store_row<T, Lines>(static_cast<char*>(L.out[to + d]) + out_row, part.col[k] * uint32_t(sizeof(T)), result, L.keep);
+                part.template store<Q8 ? 1 : sizeof(T), Lines>(results.first(to + d) + out_row, k, result.w, L.keep);
                 L.pace.wait();
             }
         }
@@ -275,10 +296,10 @@ __global__ void __launch_bounds__(256) rms_norm_narrow_kernel(const NormLaunch L
         h[c] = w[c] = 0.0f;
         if (c < L.cols) {
             for (uint32_t k = 0; k < L.nranks; ++k)
-                h[c] += load_one<T>(static_cast<const char*>(L.send[k]) + uint64_t(row) * L.send_stride + c * sizeof(T));
+                h[c] += load_one<T>(bytes_of(L.send[k]) + uint64_t(row) * L.send_stride + c * sizeof(T));
             if (L.residual[0])
-                h[c] += load_one<R>(static_cast<const char*>(L.residual[first]) + uint64_t(at) * L.residual_stride + c * sizeof(R));
-            const char* p = static_cast<const char*>(L.weight);
+                h[c] += load_one<R>(bytes_of(L.residual[first]) + uint64_t(at) * L.residual_stride + c * sizeof(R));
+            const ConstBytes p = bytes_of(L.weight);
             w[c] = L.weight32 ? load_one<float>(p + c * 4) : load_one<T>(p + c * sizeof(T));
             sum = __builtin_fmaf(h[c], h[c], sum);
             if (Q8) top = Larger()(top, magnitude(h[c] * w[c]));
@@ -290,7 +311,7 @@ __global__ void __launch_bounds__(256) rms_norm_narrow_kernel(const NormLaunch L
     const float limit = L.int8 ? kInt8Max : kE4m3Max;
     if (Q8) {
         finite = row_scale(r, top, L.int8, scale, inverse);
-        for (uint32_t d = 0; d < L.ndst; ++d) *as_global<float>(reinterpret_cast<char*>(L.scales[first + d] + at)) = scale;
+        for (uint32_t d = 0; d < L.ndst; ++d) L.scales[first + d][at] = scale;
     }
     float y[8];
 #pragma unroll
@@ -304,7 +325,7 @@ __global__ void __launch_bounds__(256) rms_norm_narrow_kernel(const NormLaunch L
         for (uint32_t c = 0; c < kNormVec; ++c)
             if (c < L.cols)
                 for (uint32_t d = 0; d < L.ndst; ++d)
-                    *as_global<uint8_t>(static_cast<char*>(L.out[first + d]) + uint64_t(at) * L.out_stride + c) =
+                    *(MRV_GLOBAL uint8_t*)(bytes_of(L.out[first + d]) + uint64_t(at) * L.out_stride + c) =
                             uint8_t(codes[c / 4] >> (8 * (c % 4)));
     }
 #pragma unroll
@@ -312,8 +333,8 @@ __global__ void __launch_bounds__(256) rms_norm_narrow_kernel(const NormLaunch L
         if (c >= L.cols) continue;
         for (uint32_t d = 0; d < L.ndst; ++d) {
             if (L.has_hidden)
-                store_one<R>(static_cast<char*>(L.hidden[first + d]) + uint64_t(at) * L.hidden_stride + c * sizeof(R), h[c]);
-            if (!Q8) store_one<T>(static_cast<char*>(L.out[first + d]) + uint64_t(at) * L.out_stride + c * sizeof(T), y[c]);
+                store_one<R>(bytes_of(L.hidden[first + d]) + uint64_t(at) * L.hidden_stride + c * sizeof(R), h[c]);
+            if (!Q8) store_one<T>(bytes_of(L.out[first + d]) + uint64_t(at) * L.out_stride + c * sizeof(T), y[c]);
         }
     }
 }
@@ -321,34 +342,36 @@ __global__ void __launch_bounds__(256) rms_norm_narrow_kernel(const NormLaunch L
 // Backward.  A row group (the lanes of one row) walks the rows of one part, `part_groups` apart, and carries its columns'
 // share of the weight's gradient in registers; the shares meet in `partial`, and norm_weight_kernel adds them in order.
 template <typename T, typename R, uint32_t Vecs, bool Wave, bool Lines, uint32_t Ranks>
-__global__ void __launch_bounds__(Wave ? 64 * kWaveRows : 1024) rms_norm_backward_kernel(const NormBackLaunch L) {
+__global__ void __launch_bounds__(Wave ? 64 * kWaveRows : 1024, 4) rms_norm_backward_kernel(const NormBackLaunch L) {
     typedef RowReduce<Wave, 2, false> Reduce;
     __shared__ typename Reduce::Shared shared;
     const uint32_t lanes = Wave ? 64 : L.lanes, lane = Wave ? threadIdx.x % 64 : threadIdx.x;
     const uint32_t group = Wave ? blockIdx.x * kWaveRows + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : blockIdx.x;
     if (Wave && group >= L.groups) return;
-    const RowPart<Vecs> part(L.cols, lanes, lane);
+    const LaneTable sends(offsetof(NormBackLaunch, send)), others(offsetof(NormBackLaunch, dsend));  // and dhidden; and hidden
+    const RowPart<Vecs, sizeof(T) == 4 || sizeof(R) == 4> part(L.cols, lanes, lane);
     const uint32_t first = group / L.part_groups;  // the destination whose rows these are (reduce_scatter); 0 (all_reduce)
+    constexpr bool kAhead = Vecs == 1;
     float w[Vecs][8], dw[Vecs][8];
-    load_weight<T, Vecs>(L.weight, L.weight32, part.col, w);
 #pragma unroll
-    for (uint32_t k = 0; k < Vecs; ++k)
+    for (uint32_t k = 0; k < Vecs; ++k) {
+        if (kAhead) load_weight<T>(L.weight, L.weight32, part, k, w[k]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) dw[k][i] = 0.0f;
+    }
     const float mean = 1.0f / float(L.cols);
-    const void* const arriving_part = L.arriving[0] ? L.arriving[first] : nullptr;
+    const ConstBytes arriving_part = bytes_of(L.arriving[0] ? L.arriving[first] : nullptr);
 
     // As in the forward kernel the next row's loads are issued before this one's stores; two vectors per lane leave
-    // no registers for that.
-    constexpr bool kAhead = Vecs == 1;
+    // no registers for that, nor for the weight, which is read again where it is used.
     FirstRanks<T, Lines, Vecs, Ranks> ahead;
-    constexpr bool kArrivingAhead = kAhead && sizeof(R) == 2;
+    constexpr bool kArrivingAhead = kAhead && sizeof(R) == 2 && Ranks < 8;
     Raw8<R> hidden[Vecs], arriving[Vecs], arriving_ahead[Vecs];
     auto send_row = [&](uint32_t at) { return (uint64_t(first) * L.part_rows + at) * L.send_stride; };
     auto fetch = [&](uint32_t at) {
-        load_row<R, Lines, Vecs>(L.hidden[first], uint64_t(at) * L.hidden_stride, part.col, hidden);
-        if (kArrivingAhead) load_row<R, Lines, Vecs>(arriving_part, uint64_t(at) * L.arriving_stride, part.col, arriving_ahead);
-        ahead.load(L.send, L.nranks, send_row(at), part.col);
+        load_row<R, Lines, Vecs>(others.second(first), uint64_t(at) * L.hidden_stride, part, hidden);
+        if (kArrivingAhead) load_row<R, Lines, Vecs>(arriving_part, uint64_t(at) * L.arriving_stride, part, arriving_ahead);
+        ahead.load(sends, L.nranks, send_row(at), part);
     };
     uint32_t slot = 0, position = group - first * L.part_groups, next = L.deal.of(position);
     if (kAhead) fetch(next);
@@ -356,14 +379,15 @@ __global__ void __launch_bounds__(Wave ? 64 * kWaveRows : 1024) rms_norm_backwar
         const uint32_t at = next;
         float g[Vecs][8], h[Vecs][8];
         if (!kAhead) fetch(at);
-        ahead.fold(L.send, L.nranks, send_row(at), part.col, g);
+        ahead.fold(sends, L.nranks, send_row(at), part, g);
         float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (uint32_t k = 0; k < Vecs; ++k) {
             widen<R>(hidden[k], h[k]);
+            if (!kAhead) load_weight<T>(L.weight, L.weight32, part, k, w[k]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float mine = uint32_t(i) >= part.repeat[k] ? h[k][i] : 0.0f;
+                const float mine = part.mine(k, uint32_t(i)) ? h[k][i] : 0.0f;
                 sum[0] = __builtin_fmaf(h[k][i], mine, sum[0]);
                 sum[1] = __builtin_fmaf(g[k][i] * w[k][i], mine, sum[1]);
             }
@@ -371,8 +395,8 @@ __global__ void __launch_bounds__(Wave ? 64 * kWaveRows : 1024) rms_norm_backwar
         if constexpr (kArrivingAhead) {
 #pragma unroll
             for (uint32_t k = 0; k < Vecs; ++k) arriving[k] = arriving_ahead[k];
-        } else {
-            load_row<R, Lines, Vecs>(arriving_part, uint64_t(at) * L.arriving_stride, part.col, arriving);
+        } else if constexpr (kAhead) {
+            load_row<R, Lines, Vecs>(arriving_part, uint64_t(at) * L.arriving_stride, part, arriving);
         }
         position += L.part_groups;
         next = L.deal.of(position);
@@ -385,30 +409,30 @@ __global__ void __launch_bounds__(Wave ? 64 * kWaveRows : 1024) rms_norm_backwar
 #pragma unroll
         for (uint32_t k = 0; k < Vecs; ++k) {
             float dh[8];
-            widen<R>(arriving[k], dh);
+            if (!kAhead) load_weight<T>(L.weight, L.weight32, part, k, w[k]);
+            if constexpr (kAhead) widen<R>(arriving[k], dh);
+            else widen<R>(arriving_part ? part.template load<R, Lines>(arriving_part + uint64_t(at) * L.arriving_stride, k) : Raw8<R>{}, dh);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 dh[i] += __builtin_fmaf(-pull, h[k][i], r * (g[k][i] * w[k][i]));
                 dw[k][i] = __builtin_fmaf(g[k][i], h[k][i] * r, dw[k][i]);
             }
-            if (!part.stores(k)) continue;
             const Raw8<R> wide = narrow<R>(dh);
             const Raw8<T> slim = narrow<T>(dh);
             for (uint32_t d = 0; d < L.ndst; ++d) {
                 if (L.dhidden[0]) {
-                    store_row<R, Lines>(static_cast<char*>(L.dhidden[first + d]) + dhidden_row, part.col[k] * uint32_t(sizeof(R)), wide, L.keep);
+                    part.template store<sizeof(R), Lines>(sends.second(first + d) + dhidden_row, k, wide.w, L.keep);
                 }
                 if (L.dsend[0]) {
-                    store_row<T, Lines>(static_cast<char*>(L.dsend[first + d]) + dsend_row, part.col[k] * uint32_t(sizeof(T)), slim, L.keep);
+                    part.template store<sizeof(T), Lines>(others.first(first + d) + dsend_row, k, slim.w, L.keep);
                 }
             }
         }
     }
     if (L.partial) {
-        char* p = reinterpret_cast<char*>(L.partial + uint64_t(group) * L.cols);
+        const Bytes p = bytes_of(L.partial + uint64_t(group) * L.cols);
 #pragma unroll
-        for (uint32_t k = 0; k < Vecs; ++k)
-            if (part.stores(k)) store8<float>(p + part.col[k] * 4, narrow<float>(dw[k]), true);
+        for (uint32_t k = 0; k < Vecs; ++k) part.template store<4, false>(p, k, narrow<float>(dw[k]).w, true);
     }
 }
 
@@ -421,7 +445,7 @@ __global__ void __launch_bounds__(256) rms_norm_backward_narrow_kernel(const Nor
     float w[kNormVec], dw[kNormVec];
 #pragma unroll
     for (uint32_t c = 0; c < kNormVec; ++c) {
-        const char* p = static_cast<const char*>(L.weight);
+        const ConstBytes p = bytes_of(L.weight);
         w[c] = c >= L.cols ? 0.0f : L.weight32 ? load_one<float>(p + c * 4) : load_one<T>(p + c * sizeof(T));
         dw[c] = 0.0f;
     }
@@ -433,10 +457,10 @@ __global__ void __launch_bounds__(256) rms_norm_backward_narrow_kernel(const Nor
             g[c] = h[c] = a[c] = 0.0f;
             if (c < L.cols) {
                 for (uint32_t k = 0; k < L.nranks; ++k)
-                    g[c] += load_one<T>(static_cast<const char*>(L.send[k]) + row * L.send_stride + c * sizeof(T));
-                h[c] = load_one<R>(static_cast<const char*>(L.hidden[first]) + uint64_t(at) * L.hidden_stride + c * sizeof(R));
+                    g[c] += load_one<T>(bytes_of(L.send[k]) + row * L.send_stride + c * sizeof(T));
+                h[c] = load_one<R>(bytes_of(L.hidden[first]) + uint64_t(at) * L.hidden_stride + c * sizeof(R));
                 if (L.arriving[0])
-                    a[c] = load_one<R>(static_cast<const char*>(L.arriving[first]) + uint64_t(at) * L.arriving_stride + c * sizeof(R));
+                    a[c] = load_one<R>(bytes_of(L.arriving[first]) + uint64_t(at) * L.arriving_stride + c * sizeof(R));
             }
             square = __builtin_fmaf(h[c], h[c], square);
             inner = __builtin_fmaf(g[c] * w[c], h[c], inner);
@@ -450,9 +474,9 @@ __global__ void __launch_bounds__(256) rms_norm_backward_narrow_kernel(const Nor
             dw[c] = __builtin_fmaf(g[c], h[c] * r, dw[c]);
             for (uint32_t d = 0; d < L.ndst; ++d) {
                 if (L.dhidden[0])
-                    store_one<R>(static_cast<char*>(L.dhidden[first + d]) + uint64_t(at) * L.dhidden_stride + c * sizeof(R), dh);
+                    store_one<R>(bytes_of(L.dhidden[first + d]) + uint64_t(at) * L.dhidden_stride + c * sizeof(R), dh);
                 if (L.dsend[0])
-                    store_one<T>(static_cast<char*>(L.dsend[first + d]) + uint64_t(at) * L.dsend_stride + c * sizeof(T), dh);
+                    store_one<T>(bytes_of(L.dsend[first + d]) + uint64_t(at) * L.dsend_stride + c * sizeof(T), dh);
             }
         }
     }
@@ -470,8 +494,8 @@ constexpr uint32_t kLongLanes = 1024;
 
 template <typename T>
 __device__ __forceinline__ void load_weight_part(const void* weight, uint32_t weight32, uint32_t col, uint32_t have, float (&w)[8]) {
-    if (weight32) load_part<float>(static_cast<const char*>(weight) + uint64_t(col) * 4, have, w);
-    else load_part<T>(static_cast<const char*>(weight) + uint64_t(col) * sizeof(T), have, w);
+    if (weight32) load_part<float>(bytes_of(weight) + uint64_t(col) * 4, have, w);
+    else load_part<T>(bytes_of(weight) + uint64_t(col) * sizeof(T), have, w);
 }
 // The fold of `have` elements at byte `offset` of every rank's buffer.
 template <typename T>
@@ -481,7 +505,7 @@ __device__ __forceinline__ void fold_part(const void* const* send, uint32_t nran
 #pragma unroll 4
     for (uint32_t k = 0; k < nranks; ++k) {
         float f[8];
-        load_part<T>(static_cast<const char*>(send[k]) + offset, have, f);
+        load_part<T>(bytes_of(send[k]) + offset, have, f);
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[i] += f[i];
     }
@@ -494,7 +518,7 @@ __global__ void __launch_bounds__(kLongLanes) rms_norm_long_kernel(const NormLau
     const uint32_t row = blockIdx.x;
     const uint32_t first = row / L.part_rows, at = row - first * L.part_rows;
     const uint64_t send_row = uint64_t(row) * L.send_stride;
-    const char* residual = L.residual[0] ? static_cast<const char*>(L.residual[first]) + uint64_t(at) * L.residual_stride : nullptr;
+    const ConstBytes residual = L.residual[0] ? bytes_of(L.residual[first]) + uint64_t(at) * L.residual_stride : nullptr;
     float sum[1] = {0.0f};
     uint32_t top = 0;
     float r = 0.0f, scale = 0.0f, inverse = 0.0f;
@@ -523,7 +547,7 @@ __global__ void __launch_bounds__(kLongLanes) rms_norm_long_kernel(const NormLau
             }
             if (L.has_hidden)
                 for (uint32_t d = 0; d < L.ndst; ++d)
-                    store_part<R>(static_cast<char*>(L.hidden[first + d]) + uint64_t(at) * L.hidden_stride + c * sizeof(R), have, h, L.keep);
+                    store_part<R>(bytes_of(L.hidden[first + d]) + uint64_t(at) * L.hidden_stride + c * sizeof(R), have, h);
             float y[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] = h[i] * r * w[i];
@@ -533,18 +557,19 @@ __global__ void __launch_bounds__(kLongLanes) rms_norm_long_kernel(const NormLau
                 u32x2 codes = L.int8 ? to_int8(y) : to_e4m3(y);
                 if (!finite) codes = L.int8 ? u32x2{0, 0} : u32x2{0x7f7f7f7fu, 0x7f7f7f7fu};
                 for (uint32_t d = 0; d < L.ndst; ++d) {
-                    char* p = static_cast<char*>(L.out[first + d]) + uint64_t(at) * L.out_stride + c;
+                    const Bytes p = bytes_of(L.out[first + d]) + uint64_t(at) * L.out_stride + c;
                     if (have == kNormVec) {
-                        store_codes(p, codes, L.keep);
+                        const uint32_t both[2] = {codes[0], codes[1]};
+                        store_dwords<8, false, 1>(p, 0, both, true);
                     } else {
 #pragma unroll
                         for (uint32_t i = 0; i < kNormVec; ++i)
-                            if (i < have) *as_global<uint8_t>(p + i) = uint8_t(codes[i / 4] >> (8 * (i % 4)));
+                            if (i < have) *(MRV_GLOBAL uint8_t*)(p + i) = uint8_t(codes[i / 4] >> (8 * (i % 4)));
                     }
                 }
             } else {
                 for (uint32_t d = 0; d < L.ndst; ++d)
-                    store_part<T>(static_cast<char*>(L.out[first + d]) + uint64_t(at) * L.out_stride + c * sizeof(T), have, y, L.keep);
+                    store_part<T>(bytes_of(L.out[first + d]) + uint64_t(at) * L.out_stride + c * sizeof(T), have, y);
             }
         }
         if (sweep == 1) break;
@@ -553,7 +578,7 @@ __global__ void __launch_bounds__(kLongLanes) rms_norm_long_kernel(const NormLau
         if (Q8) {
             finite = row_scale(r, top, L.int8, scale, inverse);
             if (threadIdx.x == 0)
-                for (uint32_t d = 0; d < L.ndst; ++d) *as_global<float>(reinterpret_cast<char*>(L.scales[first + d] + at)) = scale;
+                for (uint32_t d = 0; d < L.ndst; ++d) L.scales[first + d][at] = scale;
         }
     }
 }
@@ -567,7 +592,7 @@ __global__ void __launch_bounds__(kLongLanes) rms_norm_backward_long_kernel(cons
     uint32_t slot = 0;
     for (uint32_t at = group - first * L.part_groups; at < L.part_rows; at += L.part_groups, slot ^= 1, fresh = false) {
         const uint64_t send_row = (uint64_t(first) * L.part_rows + at) * L.send_stride;
-        const char* hidden = static_cast<const char*>(L.hidden[first]) + uint64_t(at) * L.hidden_stride;
+        const ConstBytes hidden = bytes_of(L.hidden[first]) + uint64_t(at) * L.hidden_stride;
         float sum[2] = {0.0f, 0.0f}, r = 0.0f, pull = 0.0f;
         for (uint32_t sweep = 0; sweep < 2; ++sweep) {
             for (uint64_t c = uint64_t(threadIdx.x) * kNormVec; c < L.cols; c += kLongLanes * kNormVec) {
@@ -586,23 +611,23 @@ __global__ void __launch_bounds__(kLongLanes) rms_norm_backward_long_kernel(cons
                     continue;
                 }
                 if (L.partial) {
-                    char* share = reinterpret_cast<char*>(L.partial + uint64_t(group) * L.cols + c);
+                    const Bytes share = bytes_of(L.partial + uint64_t(group) * L.cols + c);
                     float dw[8] = {};
                     if (!fresh) load_part<float>(share, have, dw);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) dw[i] = __builtin_fmaf(g[i], h[i] * r, dw[i]);
-                    store_part<float>(share, have, dw, true);
+                    store_part<float>(share, have, dw);
                 }
                 float dh[8] = {};
                 if (L.arriving[0])
-                    load_part<R>(static_cast<const char*>(L.arriving[first]) + uint64_t(at) * L.arriving_stride + c * sizeof(R), have, dh);
+                    load_part<R>(bytes_of(L.arriving[first]) + uint64_t(at) * L.arriving_stride + c * sizeof(R), have, dh);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) dh[i] += __builtin_fmaf(-pull, h[i], r * (g[i] * w[i]));
                 for (uint32_t d = 0; d < L.ndst; ++d) {
                     if (L.dhidden[0])
-                        store_part<R>(static_cast<char*>(L.dhidden[first + d]) + uint64_t(at) * L.dhidden_stride + c * sizeof(R), have, dh, L.keep);
+                        store_part<R>(bytes_of(L.dhidden[first + d]) + uint64_t(at) * L.dhidden_stride + c * sizeof(R), have, dh);
                     if (L.dsend[0])
-                        store_part<T>(static_cast<char*>(L.dsend[first + d]) + uint64_t(at) * L.dsend_stride + c * sizeof(T), have, dh, L.keep);
+                        store_part<T>(bytes_of(L.dsend[first + d]) + uint64_t(at) * L.dsend_stride + c * sizeof(T), have, dh);
                 }
             }
             if (sweep == 1) break;
@@ -625,17 +650,18 @@ NormKernels norm_kernels_of(bool q8) {
 
 template <typename T, typename R, bool Wave, bool Lines>
 NormKernels norm_kernels_ranks(uint32_t nranks, bool q8) {
-    constexpr uint32_t kMost = sizeof(T) == 4 ? 4 : 8;  // eight 16-byte loads
+    constexpr uint32_t kMost = sizeof(T) == 4 ? 4 : 8;  // 32 registers' worth
+    constexpr uint32_t kBackMost = sizeof(T) == 4 ? 4 : sizeof(R) == 4 ? 6 : 8;  // what the backward's other values leave
     if (nranks <= 2) return norm_kernels_of<T, R, 1, Wave, Lines, 2, 2>(q8);
     if (nranks <= 4) return norm_kernels_of<T, R, 1, Wave, Lines, 4, 4>(q8);
-    return norm_kernels_of<T, R, 1, Wave, Lines, kMost, kMost>(q8);
+    return norm_kernels_of<T, R, 1, Wave, Lines, kMost, kBackMost>(q8);
 }
 
 template <typename T, typename R, bool Lines>
 NormKernels norm_kernels_lines(NormVariant v, uint32_t nranks, bool q8) {
     if (v == kNormWave) return norm_kernels_ranks<T, R, true, Lines>(nranks, q8);
     if (v == kNormBlock) return norm_kernels_ranks<T, R, false, Lines>(nranks, q8);
-    return norm_kernels_of<T, R, 2, false, Lines, sizeof(T) == 4 ? 2 : 4, sizeof(T) == 4 ? 1 : 3>(q8);
+    return norm_kernels_of<T, R, 2, false, Lines, sizeof(T) == 4 ? 2 : 4, sizeof(R) == 4 ? 1 : 2>(q8);
 }
 
 template <typename T, typename R>
