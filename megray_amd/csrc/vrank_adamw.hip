@@ -38,11 +38,11 @@ struct Elements {
     }
     // `Size` bytes per element; `tile_at`: the workgroup's first element
     template <uint32_t Size, bool Lines>
-    __device__ __forceinline__ void store(Bytes base, uint64_t tile_at, const uint32_t* w) const {
+    __device__ __forceinline__ void store(Bytes base, uint64_t tile_at, const uint32_t* w, bool keep) const {
         if (whole()) {
             const Bytes tile = base + tile_at * Size;  // the same for the whole wavefront
 #pragma unroll
-            for (uint32_t p = 0; p < 2; ++p) store_dwords<4 * Size, Lines, Size>(tile, uint32_t(at[p] - tile_at) * Size, w + p * Size, false);
+            for (uint32_t p = 0; p < 2; ++p) store_dwords<4 * Size, Lines, Size>(tile, uint32_t(at[p] - tile_at) * Size, w + p * Size, keep);
         } else {
 #pragma unroll
             for (uint32_t i = 0; i < 8; ++i) {
@@ -99,7 +99,7 @@ __device__ __forceinline__ uint32_t to_block(const float* x, float& scale) {
     float amax = __builtin_bit_cast(float, across_wave(top, Larger()));
     if (amax < kAmaxMin) amax = kAmaxMin;  // not true of a NaN
     const bool finite = amax < __builtin_inff();
-    scale = amax / kE4m3Max;
+    scale = amax * (1.0f / kE4m3Max);
     const float inverse = 1.0f / scale;
     float q[4];
 #pragma unroll
@@ -183,10 +183,10 @@ __device__ __forceinline__ void adamw_tile(const AdamLaunch& L, const AdamTensor
         const float update = L.rate * m[j] / __builtin_fmaf(root[j], L.root_scale, L.eps);
         p[j] = __builtin_fmaf(-shrink, p[j], p[j]) - update;
     }
-    e.store<4, Lines>(bytes_of(t.master), tile_at, narrow<float>(p).w);
+    e.store<4, Lines>(bytes_of(t.master), tile_at, narrow<float>(p).w, L.keep);
     const Raw8<P> param = narrow<P>(p);
     for (uint32_t r = 0; r < L.param_ranks; ++r)
-        e.store<sizeof(P), Lines>(bytes_of(L.params[uint64_t(tensor) * L.param_ranks + r]), tile_at, param.w);
+        e.store<sizeof(P), Lines>(bytes_of(L.params[uint64_t(tensor) * L.param_ranks + r]), tile_at, param.w, L.keep);
     if constexpr (State8) {
 #pragma unroll
         for (uint32_t j = 0; j < 8; ++j)  // elements behind the tensor's end do not count for the block's maximum
@@ -200,11 +200,11 @@ __device__ __forceinline__ void adamw_tile(const AdamLaunch& L, const AdamTensor
                 store_one<float>(bytes_of(t.v_scale + block + q), v_scale[q]);
             }
         }
-        e.store<1, Lines>(bytes_of(t.m), tile_at, m_codes);
-        e.store<1, Lines>(bytes_of(t.v), tile_at, v_codes);
+        e.store<1, Lines>(bytes_of(t.m), tile_at, m_codes, L.keep);
+        e.store<1, Lines>(bytes_of(t.v), tile_at, v_codes, L.keep);
     } else {
-        e.store<4, Lines>(bytes_of(t.m), tile_at, narrow<float>(m).w);
-            e.store<4, Lines>(bytes_of(t.v), tile_at, narrow<float>(v).w);
+        e.store<4, Lines>(bytes_of(t.m), tile_at, narrow<float>(m).w, L.keep);
+            e.store<4, Lines>(bytes_of(t.v), tile_at, narrow<float>(v).w, L.keep);
     }
 }
 

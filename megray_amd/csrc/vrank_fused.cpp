@@ -524,6 +524,9 @@ Adamw::Adamw(const mrv_adamw_tensors& t) {
     }
     check_intervals(used);
 
+    uint64_t written = 0;
+    for (const Interval& x : used) written += x.written ? x.end - x.begin : 0;
+    m_step.keep = written <= kKeepMaxBytes;
     m_groups = uint32_t(std::min<uint64_t>(ntiles, kAdamNormGroups));
     if (hipGetDevice(&m_device) != hipSuccess) {
         (void)hipGetLastError();

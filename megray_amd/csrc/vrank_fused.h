@@ -161,6 +161,7 @@ struct AdamLaunch {
     uint32_t grad_ranks, param_ranks;
     uint32_t ntiles;
     Deal deal;  // of the tiles
+    uint32_t keep;  // stores leave their data in the last-level cache
     float lr, beta1, beta2, eps;
     float rest1, rest2;  // 1 - beta1, 1 - beta2, from 64 bits: a beta near 1 has few bits of them left
     float rate;        // lr / (1 - beta1^step)

@@ -6,7 +6,9 @@
 
 #include <hip/hip_runtime.h>
 
+#include <cstddef>
 #include <cstdint>
+#include <type_traits>
 
 #include "vrank_fused.h"
 
@@ -270,16 +272,31 @@ __device__ __forceinline__ uint32_t magnitude(float x) {
 
 // ---- over the lanes of a wavefront ---------------------------------------------------------------
 
+// Sixteen lanes' values combined, the same bits in each of them: by rotations, after the step of n lanes the values repeat
+// every n, so that a lane combines the same pairs as its neighbours.
 template <typename V, typename Op>
-__device__ __forceinline__ V across_half(V x, Op op) {  // over 32 lanes, the same in each of them
-#pragma unroll
-    for (int d = 16; d; d >>= 1) x = op(x, __shfl_xor(x, d, 64));
-    return x;
+__device__ __forceinline__ V across_row(V x, Op op) {
+    auto turned = [](V v, auto n) {
+        const int i = __builtin_bit_cast(int, v);
+        return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(i, i, 0x120 + decltype(n)::value, 0xf, 0xf, false));  // row_ror:n
+    };
+    x = op(x, turned(x, std::integral_constant<int, 8>()));
+    x = op(x, turned(x, std::integral_constant<int, 4>()));
+    x = op(x, turned(x, std::integral_constant<int, 2>()));
+    return op(x, turned(x, std::integral_constant<int, 1>()));
 }
+// All 64 lanes' values: the four rows through scalar registers.
 template <typename V, typename Op>
 __device__ __forceinline__ V across_wave(V x, Op op) {
-    x = across_half(x, op);
-    return op(x, __shfl_xor(x, 32, 64));
+    if constexpr (sizeof(V) == 4) {
+        x = across_row(x, op);
+        auto row = [&](int lane) { return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane)); };
+        return op(op(row(0), row(16)), op(row(32), row(48)));
+    } else {
+#pragma unroll
+        for (int d = 32; d; d >>= 1) x = op(x, __shfl_xor(x, d, 64));
+        return x;
+    }
 }
 struct Plus {
     template <typename V>

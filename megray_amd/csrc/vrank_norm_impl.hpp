@@ -43,12 +43,12 @@ struct RowReduce {
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < Sums; ++i) {
-                sum[i] = s.sum[slot][i][0];
-                for (uint32_t w = 1; w < waves; ++w) sum[i] += s.sum[slot][i][w];
+                const float part = s.sum[slot][i][threadIdx.x % 16];  // anything, where there is no such wavefront
+                sum[i] = across_row(threadIdx.x % 16 < waves ? part : 0.0f, Plus());
             }
             if (Max) {
-                max = s.max[slot][0];
-                for (uint32_t w = 1; w < waves; ++w) max = Larger()(max, s.max[slot][w]);
+                const uint32_t part = s.max[slot][threadIdx.x % 16];
+                max = across_row(threadIdx.x % 16 < waves ? part : 0u, Larger());
             }
         }
     }
@@ -179,7 +179,7 @@ __device__ __forceinline__ void load_row(ConstBytes ptr, uint64_t row_offset, co
 __device__ __forceinline__ bool row_scale(float r, uint32_t top, uint32_t int8, float& scale, float& inverse) {
     float amax = r * __builtin_bit_cast(float, top);
     if (amax < kAmaxMin) amax = kAmaxMin;  // not true of a NaN
-    scale = amax / (int8 ? kInt8Max : kE4m3Max);
+    scale = amax * (int8 ? 1.0f / kInt8Max : 1.0f / kE4m3Max);
     inverse = 1.0f / scale;
     if (amax < __builtin_inff()) return true;
     scale = __builtin_nanf("");
