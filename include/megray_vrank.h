@@ -488,7 +488,7 @@ MRV_API void mrv_adamw_destroy(mrv_adamw* handle);
 /*
  * The norm of all folded gradients, g = grad_scale * sum over k of grads[k]:
  *   out[0] = sqrt(sum of g * g),   out[1] = min(1, max_norm / (out[0] + 1e-6)), or NaN where the norm is not finite.
- * Squares are summed in 64 bits.  `out` is device memory of mrv_adamw_norm_floats() floats, aligned to 8; what follows
+ * Squares are summed in 64 bits.  `out`, apart from the handle's tensors, is device memory of mrv_adamw_norm_floats() floats, aligned to 8; what follows
  * out[1] is scratch.  Calls that may run at the same time need an `out` each.
  */
 MRV_API size_t mrv_adamw_norm_floats(const mrv_adamw* handle);
@@ -498,7 +498,7 @@ MRV_API int mrv_adamw_grad_norm(const mrv_adamw* handle, float grad_scale, float
  * One step, with g = grad_scale * *clip * sum over k of grads[k] (clip: a float in device memory, out + 1 of the call above say; null: 1):
  *   m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g g,
  *   p = p (1 - lr weight_decay) - lr (m / (1 - beta1^step)) / (sqrt(v / (1 - beta2^step)) + eps)
- * in 32 bits; params get p rounded to their type.  A step whose *clip is not finite changes nothing.  `step` counts from 1.  The
+ * in 32 bits; params get p rounded to their type.  `clip` is not part of what the step writes.  A step whose *clip is not finite changes nothing.  `step` counts from 1.  The
  * numbers are arguments of the launch: a step captured into a graph repeats them.
  */
 typedef struct mrv_adamw_step_args {

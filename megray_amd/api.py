@@ -522,17 +522,20 @@ class AdamWPlan:
             grad_ranks=len(grads), param_ranks=0 if params is None else len(params), grad_dtype=int(grad_dtype),
             param_dtype=int(grad_dtype if param_dtype is None else param_dtype), state_dtype=int(state_dtype))
         _check(_lib.load().mrv_adamw_create(call, ctypes.byref(self._h)))
+        self._norm_bytes = 4 * _lib.load().mrv_adamw_norm_floats(self._h)
         self._step = _lib.load().mrv_adamw_step
         self._norm = _lib.load().mrv_adamw_grad_norm
 
     @property
     def norm_floats(self):
         """Floats that grad_norm()'s `out` has to hold."""
-        return _lib.load().mrv_adamw_norm_floats(self._h)
+        return self._norm_bytes // 4
 
     def grad_norm(self, out, grad_scale=1.0, max_norm=float("inf"), stream=None):
         """out[0] = the norm of grad_scale * the folded gradients, out[1] = min(1, max_norm / (norm + 1e-6)), NaN where the norm is
         not finite; what follows is scratch (mrv_adamw_grad_norm)."""
+        if hasattr(out, "numel") and out.numel() * out.element_size() < self._norm_bytes:
+            raise MegRayError(Status.INVALID_ARGUMENT, f"out has to hold {self.norm_floats} floats")
         status = self._norm(self._h, grad_scale, max_norm, _ptr(out), _stream(stream))
         if status:
             _check(status)

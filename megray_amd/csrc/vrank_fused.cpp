@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <iterator>
 #include <new>
 
 #include "megray/hip_context.h"
@@ -428,18 +429,27 @@ struct Interval {
     bool written;
 };
 
-// No output may overlap anything else.
-void check_intervals(std::vector<Interval>& all) {
+// No output may overlap anything else.  Returns what is taken by all tensors and by those that are written.
+void check_intervals(std::vector<Interval>& all, Taken& any, Taken& written) {
     std::sort(all.begin(), all.end(), [](const Interval& a, const Interval& b) { return a.begin < b.begin; });
-    uintptr_t end_any = 0, end_written = 0;
     for (const Interval& x : all) {
-        if (x.begin < (x.written ? end_any : end_written)) MEGRAY_THROW("a tensor that is written overlaps another");
-        end_any = std::max(end_any, x.end);
-        if (x.written) end_written = std::max(end_written, x.end);
+        if ((x.written ? any : written).overlaps(x.begin, x.end)) MEGRAY_THROW("a tensor that is written overlaps another");
+        any.add(x.begin, x.end);
+        if (x.written) written.add(x.begin, x.end);
     }
 }
 
 }  // namespace
+
+void Taken::add(uintptr_t begin, uintptr_t end) {
+    if (!m_runs.empty() && begin <= m_runs.back().second) m_runs.back().second = std::max(m_runs.back().second, end);
+    else m_runs.push_back({begin, end});
+}
+
+bool Taken::overlaps(uintptr_t begin, uintptr_t end) const {
+    auto next = std::lower_bound(m_runs.begin(), m_runs.end(), end, [](const std::pair<uintptr_t, uintptr_t>& run, uintptr_t at) { return run.first < at; });
+    return next != m_runs.begin() && std::prev(next)->second > begin;  // the last run that begins before `end`
+}
 
 Adamw::Adamw(const mrv_adamw_tensors& t) {
     if (t.grad_ranks < 1 || t.grad_ranks > kMaxRanks) MEGRAY_THROW("grad_ranks must be in [1, 32]");
@@ -522,7 +532,7 @@ Adamw::Adamw(const mrv_adamw_tensors& t) {
             take(x.v_scale, blocks * 4, 4, true, "a scale buffer is null");
         }
     }
-    check_intervals(used);
+    check_intervals(used, m_any, m_written);
 
     uint64_t written = 0;
     for (const Interval& x : used) written += x.written ? x.end - x.begin : 0;
@@ -577,6 +587,7 @@ Status Adamw::grad_norm(float grad_scale, float max_norm, float* out, hipStream_
     if (reinterpret_cast<uintptr_t>(out) % 8) MEGRAY_THROW("out does not lie on a multiple of 8 bytes");
     if (!std::isfinite(grad_scale)) MEGRAY_THROW("grad_scale is not finite");
     if (!(max_norm >= 0.0f)) MEGRAY_THROW("max_norm must not be negative");
+    if (m_any.overlaps(reinterpret_cast<uintptr_t>(out), reinterpret_cast<uintptr_t>(out + norm_floats()))) MEGRAY_THROW("out overlaps a tensor");
     check_device();
     AdamNormLaunch L = m_norm;
     L.grad_scale = grad_scale;
@@ -594,6 +605,8 @@ Status Adamw::step(const mrv_adamw_step_args& a, hipStream_t stream) const {
     if (!(a.eps >= 0) || !std::isfinite(float(a.eps))) MEGRAY_THROW("eps must be finite and not negative");
     if (a.step < 1) MEGRAY_THROW("step counts from 1");
     if (reinterpret_cast<uintptr_t>(a.clip) % 4) MEGRAY_THROW("clip does not lie on a multiple of 4 bytes");
+    if (a.clip && m_written.overlaps(reinterpret_cast<uintptr_t>(a.clip), reinterpret_cast<uintptr_t>(a.clip + 1)))
+        MEGRAY_THROW("clip lies in a tensor that the step writes");
     check_device();
     AdamLaunch L = m_step;
     L.lr = float(a.lr);

@@ -14,6 +14,7 @@
 
 #include <cstdint>
 #include <memory>
+#include <utility>
 #include <vector>
 
 #include "megray_vrank.h"
@@ -218,6 +219,16 @@ private:
 // Bytes of workspace a backward with weight gradients needs.
 size_t norm_backward_workspace(int collective, uint32_t nranks, size_t rows, size_t cols);
 
+// Address ranges, added in the order of their beginnings.
+class Taken {
+public:
+    void add(uintptr_t begin, uintptr_t end);
+    bool overlaps(uintptr_t begin, uintptr_t end) const;
+
+private:
+    std::vector<std::pair<uintptr_t, uintptr_t>> m_runs;  // apart, ascending
+};
+
 class Adamw {
 public:
     // Checks the tensors and uploads their tables (device allocation, synchronous).
@@ -236,6 +247,7 @@ private:
     int m_device = 0;
     uint32_t m_groups = 0;
     bool m_can_step = false;
+    Taken m_any, m_written;  // by the tensors
     AdamLaunch m_step{};
     AdamNormLaunch m_norm{};
     const void* m_step_kernel = nullptr;
