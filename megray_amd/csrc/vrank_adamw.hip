@@ -18,8 +18,8 @@ using namespace fused;
 struct Elements {
     uint64_t at[2];    // first element of each piece of four
     uint32_t have[2];  // how many of the four are there
-    __device__ __forceinline__ Elements(uint32_t tile, uint64_t len) {
-        const uint64_t first = uint64_t(tile) * kAdamTile + threadIdx.x / 64 * 512u + threadIdx.x % 64 * 4u;
+    __device__ __forceinline__ Elements(uint64_t tile_at, uint64_t len) {  // the workgroup's first element
+        const uint64_t first = tile_at + threadIdx.x / 64 * 512u + threadIdx.x % 64 * 4u;
 #pragma unroll
         for (uint32_t p = 0; p < 2; ++p) {
             at[p] = first + p * kAdamBlock;
@@ -111,11 +111,14 @@ __device__ __forceinline__ uint32_t to_block(const float* x, float& scale) {
     return finite ? to_e4m3(q[0], q[1], q[2], q[3]) : 0x7f7f7f7fu;
 }
 
+template <bool State8>
+constexpr uint32_t kThreads = State8 ? kAdamThreads8 : kAdamThreads;
+
 // Lines: the tensor's buffers all begin on a cache line.
 template <typename G, typename P, bool State8, bool Lines>
 __device__ __forceinline__ void adamw_tile(const AdamLaunch& L, const AdamTensor& t, uint32_t tensor, uint32_t tile, float factor) {
-    const Elements e(tile, t.len);
-    const uint64_t tile_at = uint64_t(tile) * kAdamTile;
+    const uint64_t tile_at = uint64_t(tile) * (kThreads<State8> * kAdamVec);
+    const Elements e(tile_at, t.len);
     const uint64_t block = tile_at / kAdamBlock + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * 2;
 
     float g[8], m[8], v[8], p[8];
@@ -184,9 +187,12 @@ __device__ __forceinline__ void adamw_tile(const AdamLaunch& L, const AdamTensor
         p[j] = __builtin_fmaf(-shrink, p[j], p[j]) - update;
     }
     e.store<4, Lines>(bytes_of(t.master), tile_at, narrow<float>(p).w, L.keep);
+    L.pace.wait();
     const Raw8<P> param = narrow<P>(p);
-    for (uint32_t r = 0; r < L.param_ranks; ++r)
+    for (uint32_t r = 0; r < L.param_ranks; ++r) {
         e.store<sizeof(P), Lines>(bytes_of(L.params[uint64_t(tensor) * L.param_ranks + r]), tile_at, param.w, L.keep);
+        L.pace.wait();
+    }
     if constexpr (State8) {
 #pragma unroll
         for (uint32_t j = 0; j < 8; ++j)  // elements behind the tensor's end do not count for the block's maximum
@@ -204,12 +210,13 @@ __device__ __forceinline__ void adamw_tile(const AdamLaunch& L, const AdamTensor
         e.store<1, Lines>(bytes_of(t.v), tile_at, v_codes, L.keep);
     } else {
         e.store<4, Lines>(bytes_of(t.m), tile_at, narrow<float>(m).w, L.keep);
-            e.store<4, Lines>(bytes_of(t.v), tile_at, narrow<float>(v).w, L.keep);
+        L.pace.wait();
+        e.store<4, Lines>(bytes_of(t.v), tile_at, narrow<float>(v).w, L.keep);
     }
 }
 
 template <typename G, typename P, bool State8>
-__global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const AdamLaunch L) {
+__global__ void __launch_bounds__(kThreads<State8>) adamw_kernel(const AdamLaunch L) {
     float factor = L.grad_scale;
     if (L.clip) {
         const float clip = *L.clip;
@@ -237,11 +244,11 @@ __device__ __forceinline__ double workgroup_sum(double x) {
 
 // Squares are summed in 64 bits: no gradient that is finite in 32 bits overflows, and the number of terms does not matter.
 template <typename G>
-__global__ void __launch_bounds__(kAdamThreads) adamw_norm_kernel(const AdamNormLaunch L) {
+__global__ void __launch_bounds__(kAdamNormThreads) adamw_norm_kernel(const AdamNormLaunch L) {
     double sum = 0.0;
     for (uint32_t n = blockIdx.x; n < L.ntiles; n += L.groups) {
         const AdamTile where = L.tiles[L.deal.of(n)];
-        const Elements e(where.tile, L.tensors[where.tensor].len);
+        const Elements e(uint64_t(where.tile) * (kAdamNormThreads * kAdamVec), L.tensors[where.tensor].len);
         float g[8];
         fold_grads<G, true>(L.grads + uint64_t(where.tensor) * L.grad_ranks, L.grad_ranks, e, g);
 #pragma unroll
@@ -250,7 +257,7 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_norm_kernel(const AdamNorm
             sum = __builtin_fma(x, x, sum);
         }
     }
-    sum = workgroup_sum<kAdamThreads>(sum);
+    sum = workgroup_sum<kAdamNormThreads>(sum);
     if (threadIdx.x == 0) reinterpret_cast<double*>(L.out + 2)[blockIdx.x] = sum;
 }
 

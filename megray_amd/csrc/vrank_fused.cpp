@@ -469,21 +469,27 @@ Adamw::Adamw(const mrv_adamw_tensors& t) {
     }
     const uint32_t param_ranks = m_can_step ? t.param_ranks : 0;
 
-    uint64_t ntiles = 0;
+    // The norm's tiles and the step's, which may be larger ones.
+    const uint32_t threads = state8 ? kAdamThreads8 : kAdamThreads;
+    const uint64_t norm_tile = kAdamNormThreads * kAdamVec, step_tile = uint64_t(threads) * kAdamVec;
+    uint64_t norm_tiles = 0, step_tiles = 0;
     for (size_t n = 0; n < t.ntensors; ++n) {
         if (t.lens[n] > (uint64_t(1) << 40)) MEGRAY_THROW("a tensor is too long");
-        ntiles += (t.lens[n] + kAdamTile - 1) / kAdamTile;
-        // a grid counts its lanes in 32 bits
-        if (ntiles >= (uint64_t(1) << 24)) MEGRAY_THROW("too many elements for one handle");
+        norm_tiles += (t.lens[n] + norm_tile - 1) / norm_tile;
+        step_tiles += m_can_step ? (t.lens[n] + step_tile - 1) / step_tile : 0;
+        // a grid counts its lanes in 32 bits, and a tensor may be a tile of a few elements
+        if (norm_tiles >= (uint64_t(1) << 24) || step_tiles * threads >= uint64_t(1) << 32) MEGRAY_THROW("too many elements for one handle");
     }
     if (t.ntensors >= (uint64_t(1) << 24)) MEGRAY_THROW("too many tensors for one handle");
 
-    // one table: tensors, tiles, gradient pointers, parameter pointers
-    const size_t tensors_bytes = t.ntensors * sizeof(AdamTensor), tiles_bytes = size_t(ntiles) * sizeof(AdamTile);
+    // one table: tensors, the norm's tiles, the step's tiles, gradient pointers, parameter pointers
+    const size_t tensors_bytes = t.ntensors * sizeof(AdamTensor);
+    const size_t norm_bytes = size_t(norm_tiles) * sizeof(AdamTile), tiles_bytes = norm_bytes + size_t(step_tiles) * sizeof(AdamTile);
     const size_t grads_bytes = t.ntensors * t.grad_ranks * sizeof(void*), params_bytes = t.ntensors * param_ranks * sizeof(void*);
     std::vector<char> host(tensors_bytes + tiles_bytes + grads_bytes + params_bytes);
     auto* tensors = reinterpret_cast<AdamTensor*>(host.data());
-    auto* tiles = reinterpret_cast<AdamTile*>(host.data() + tensors_bytes);
+    auto* norm_at = reinterpret_cast<AdamTile*>(host.data() + tensors_bytes);
+    auto* step_at = norm_at + norm_tiles;
     auto* grads = reinterpret_cast<const void**>(host.data() + tensors_bytes + tiles_bytes);
     auto* params = reinterpret_cast<void**>(host.data() + tensors_bytes + tiles_bytes + grads_bytes);
     std::vector<Interval> used;
@@ -494,7 +500,6 @@ Adamw::Adamw(const mrv_adamw_tensors& t) {
         used.push_back({a, a + bytes, written});
         bits |= a;
     };
-    size_t tile = 0;
     for (size_t n = 0; n < t.ntensors; ++n) {
         const uint64_t len = t.lens[n];
         AdamTensor& x = tensors[n];
@@ -502,7 +507,8 @@ Adamw::Adamw(const mrv_adamw_tensors& t) {
         x.len = len;
         if (!len) continue;
         bits = 0;
-        for (uint64_t k = 0; k * kAdamTile < len; ++k) tiles[tile++] = {uint32_t(n), uint32_t(k)};
+        for (uint64_t k = 0; k * norm_tile < len; ++k) *norm_at++ = {uint32_t(n), uint32_t(k)};
+        for (uint64_t k = 0; m_can_step && k * step_tile < len; ++k) *step_at++ = {uint32_t(n), uint32_t(k)};
         for (uint32_t r = 0; r < t.grad_ranks; ++r) {
             const void* p = t.grads[size_t(r) * t.ntensors + n];
             take(p, len * grad_elem, grad_elem, false, "a gradient is null");
@@ -537,7 +543,8 @@ Adamw::Adamw(const mrv_adamw_tensors& t) {
     uint64_t written = 0;
     for (const Interval& x : used) written += x.written ? x.end - x.begin : 0;
     m_step.keep = written <= kKeepMaxBytes;
-    m_groups = uint32_t(std::min<uint64_t>(ntiles, kAdamNormGroups));
+    m_step.pace.on = !state8 && written >= kLongBytes;
+    m_groups = uint32_t(std::min<uint64_t>(norm_tiles, kAdamNormGroups));
     if (hipGetDevice(&m_device) != hipSuccess) {
         (void)hipGetLastError();
         throw HipFailure();
@@ -557,14 +564,18 @@ Adamw::Adamw(const mrv_adamw_tensors& t) {
     }
     const char* table = static_cast<const char*>(m_table);
     m_norm.tensors = m_step.tensors = reinterpret_cast<const AdamTensor*>(table);
-    m_norm.tiles = m_step.tiles = reinterpret_cast<const AdamTile*>(table + tensors_bytes);
+    m_norm.tiles = reinterpret_cast<const AdamTile*>(table + tensors_bytes);
+    m_step.tiles = reinterpret_cast<const AdamTile*>(table + tensors_bytes + norm_bytes);
     m_norm.grads = m_step.grads = reinterpret_cast<const void* const*>(table + tensors_bytes + tiles_bytes);
     m_step.params = reinterpret_cast<void* const*>(const_cast<char*>(table) + tensors_bytes + tiles_bytes + grads_bytes);
     m_norm.grad_ranks = m_step.grad_ranks = t.grad_ranks;
     m_step.param_ranks = param_ranks;
-    m_norm.ntiles = m_step.ntiles = uint32_t(ntiles);
+    m_norm.ntiles = uint32_t(norm_tiles);
+    m_step.ntiles = uint32_t(step_tiles);
+    m_threads = threads;
     m_norm.groups = m_groups;
-    m_norm.deal = m_step.deal = deal_blocks(uint32_t(ntiles), uint64_t(kAdamTile) * grad_elem);
+    m_norm.deal = deal_blocks(m_norm.ntiles, norm_tile * grad_elem);
+    m_step.deal = deal_blocks(m_step.ntiles, step_tile * grad_elem);
     m_norm_kernel = adamw_norm_kernel_for(t.grad_dtype);
     if (m_can_step) m_step_kernel = adamw_kernel_for(t.grad_dtype, t.param_dtype, state8);
 }
@@ -593,7 +604,7 @@ Status Adamw::grad_norm(float grad_scale, float max_norm, float* out, hipStream_
     L.grad_scale = grad_scale;
     L.max_norm = max_norm;
     L.out = out;
-    const Status st = launch_kernel(m_norm_kernel, dim3(m_groups), kAdamThreads, &L, stream);
+    const Status st = launch_kernel(m_norm_kernel, dim3(m_groups), kAdamNormThreads, &L, stream);
     if (st != MEGRAY_OK) return st;
     return launch_kernel(adamw_norm_join_kernel(), dim3(1), kAdamJoinThreads, &L, stream);
 }
@@ -619,7 +630,7 @@ Status Adamw::step(const mrv_adamw_step_args& a, hipStream_t stream) const {
     L.root_scale = float(1 / std::sqrt(1 - std::pow(a.beta2, double(a.step))));
     L.grad_scale = float(a.grad_scale);
     L.clip = a.clip;
-    return launch_kernel(m_step_kernel, dim3(L.ntiles), kAdamThreads, &L, stream);
+    return launch_kernel(m_step_kernel, dim3(L.ntiles), m_threads, &L, stream);
 }
 
 }  // namespace vrank

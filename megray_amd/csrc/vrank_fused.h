@@ -132,9 +132,10 @@ const void* norm_weight_kernel();  // grid: 64 columns each, parts
 
 // ---- AdamW over many tensors -------------------------------------------------------------------
 
-constexpr uint32_t kAdamThreads = 256;
-constexpr uint32_t kAdamVec = 8;                           // elements of a lane
-constexpr uint32_t kAdamTile = kAdamThreads * kAdamVec;    // elements of a workgroup
+constexpr uint32_t kAdamVec = 8;               // elements of a lane
+constexpr uint32_t kAdamThreads = 1024;        // of the step with 32-bit states
+constexpr uint32_t kAdamThreads8 = 256;        // of the step with 8-bit states
+constexpr uint32_t kAdamNormThreads = 256;     // of the gradient norm
 constexpr uint32_t kAdamBlock = 256;                       // elements that share a scale of an 8-bit state: half a wavefront's
 constexpr uint32_t kAdamNormGroups = 512;                  // workgroups of the gradient norm, at most
 
@@ -149,7 +150,7 @@ struct AdamTensor {  // one per tensor, in device memory
     uint32_t lines;  // every buffer of the tensor begins on a cache line
 };
 
-struct AdamTile {
+struct AdamTile {  // what a workgroup takes at a time: as many elements as its lanes hold
     uint32_t tensor;
     uint32_t tile;  // within the tensor
 };
@@ -163,6 +164,7 @@ struct AdamLaunch {
     uint32_t ntiles;
     Deal deal;  // of the tiles
     uint32_t keep;  // stores leave their data in the last-level cache
+    Pace pace;
     float lr, beta1, beta2, eps;
     float rest1, rest2;  // 1 - beta1, 1 - beta2, from 64 bits: a beta near 1 has few bits of them left
     float rate;        // lr / (1 - beta1^step)
@@ -245,7 +247,7 @@ private:
     void check_device() const;
     void* m_table = nullptr;  // device
     int m_device = 0;
-    uint32_t m_groups = 0;
+    uint32_t m_groups = 0, m_threads = 0;
     bool m_can_step = false;
     Taken m_any, m_written;  // by the tensors
     AdamLaunch m_step{};
