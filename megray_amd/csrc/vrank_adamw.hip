@@ -2,9 +2,14 @@
 //
 // Both are one pass over the ranks' gradients, which are summed on the way: N reads of a gradient, and for the step one read
 // and one write of master, m and v and N writes of the parameter - 4 to 7 bytes per operation, HBM bound.  A workgroup
-// takes kAdamTile elements of one tensor (a table says which); a wavefront takes 512 of them, a lane two pieces of four,
-// 256 apart (see Raw8).  So a piece of a wavefront is just the 256 elements that share the scale of an 8-bit state: their
-// maximum is one reduction across it, and the new codes leave from the same registers.
+// takes a tile of one tensor (a table says which); a wavefront takes 512 elements, a lane two pieces of four, 256 apart (see
+// Raw8).  So a piece of a wavefront is just the 256 elements that share the scale of an 8-bit state: their maximum is
+// one reduction across it, and the new codes leave from the same registers.
+//
+// Measured, BF16 gradients and parameters: 8 ranks, 98 M parameters, 32-bit states 1037 us (5.5 GB, 5.31 TB/s); 1 rank, 157 M 709 us (6.21
+// TB/s); 4 ranks, 50 M in tensors that begin off the cache lines, 8-bit states 274 us (5.2 TB/s); the norm of 8 ranks' 98 M 236 us (6.7 TB/s).  A
+// step that walks its tiles and loads the next one before it stores this one is slower (1215 us: it leaves fewer wavefronts), and so are
+// half the loads in flight (1108 us), tiles of a workgroup 32 apart (1196) and stores whose ranks begin elsewhere in each tile (1045).
 #include "vrank_fused_impl.hpp"
 
 namespace MegRay {

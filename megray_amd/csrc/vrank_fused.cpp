@@ -120,6 +120,10 @@ Shape check_shape(int collective, uint32_t nranks, size_t rows, size_t cols, int
 
 // ---- how a norm is laid out --------------------------------------------------------------------
 
+// A wavefront to a row up to 512 elements against a workgroup of one wavefront: 65536 x 128 BF16 of 8 ranks 163 and 187 us, 16384 x 509 of 8 ranks
+// 96 and 117, 40000 x 504 of 1 rank 31.5 and 32.6 (backward 51.4 and 51.8); at 512 itself they are level (24.4 and 24.6, 16384 rows of
+// 8 ranks 78 and 80, backward 75 and 66).  One vector per lane up to 8192 against two: 4096 x 8192 of 8 ranks 286 and 321 us, of 2 ranks 88 and
+// 104, backward 76 and 85.  Two up to 16384 against the row swept twice: 4096 x 16384 of 8 ranks 611 and 782, backward 467 and 744.
 NormVariant norm_variant(uint32_t cols) {
     if (cols < kNormVec) return kNormNarrow;
     if (cols <= 64 * kNormVec) return kNormWave;
@@ -146,14 +150,17 @@ Layout norm_layout(NormVariant v, uint32_t cols) {
 constexpr uint32_t kComputeUnits = 256;
 
 // Workgroups that the device holds at a time, by the registers of the kernels for so many ranks (norm_kernels_ranks in
-// vrank_norm_impl.hpp): a walk over rows with more of them than that would run its second half after its first.
+// vrank_norm_impl.hpp): a walk over rows with more of them than that would run its second half after its first.  (Twice as many and half
+// as many: 8192 x 8192 BF16 of 8 ranks, forward, 575 -> 579, 575 us, backward 423 -> 423, 424; 2048 x 4096 of 4 ranks 35.9 -> 36.2, 36.0, backward
+// 35.2 -> 39.6, 33.3.)
 uint32_t resident(uint32_t lanes, uint32_t nranks, bool stream32, bool backward) {
     const uint32_t waves = backward ? (nranks <= 2 ? 20 : 16) : nranks <= 2 ? 24 : nranks <= 4 && !stream32 ? 20 : 16;
     return kComputeUnits * std::max(1u, waves * 64 / lanes);
 }
 
 // Row groups of a backward, per part: enough to fill the device and no more than twice that, sixteen rows to each if there are (a group
-// writes its share of the weight's gradient once), as many to each as to the others.
+// writes its share of the weight's gradient once), as many to each as to the others.  (Eight rows to each and 32: 8192 x 8192 BF16 of 8 ranks 423 ->
+// 422, 429 us, of 2 ranks 145 -> 145, 142; up to once and four times what the device holds: 427, 423, and 141, 145.)
 uint32_t backward_groups(NormVariant v, uint32_t cols, uint32_t part_rows, uint32_t nranks, uint32_t nparts) {
     if (!part_rows) return 0;
     const Layout layout = norm_layout(v, cols);
@@ -164,8 +171,40 @@ uint32_t backward_groups(NormVariant v, uint32_t cols, uint32_t part_rows, uint3
     return (part_rows + each - 1) / each;
 }
 
-constexpr uint64_t kLongBytes = uint64_t(256) << 20;  // written in all, from which a launch is a long one
-constexpr uint32_t kDealBytes = 256 << 10;  // of a buffer that an XCD writes in one run
+// Written in all, from which a launch is a long one: its stores go one at a time.  Off and on, rows of 8192 BF16 with the hidden state:
+// 16384 of 2 ranks 367 -> 344 us, 8192 of 4 ranks 315 -> 306, 8192 of 8 ranks 581 -> 575; below, 1024 of 8 ranks, nothing (76 and 76).
+// AdamW with 32-bit states: 1 rank, 2.2 GB written, 737 -> 709 us, 352 MB 119.6 -> 118.0; 8 ranks, 2.7 GB 1052 -> 1037, 704 MB 281 -> 279,
+// 352 MB 149 -> 151; below, 1 rank, 176 MB, 62.4 -> 62.7, 8 ranks, 88 MB, 34.9 -> 35.8.
+constexpr uint64_t kLongBytes = uint64_t(256) << 20;
+
+// Whether each row has a workgroup of its own, or the workgroups that the device holds walk the rows, each loading its next row before it
+// stores this one.  Rows so wide that a CU holds one workgroup need the walk (8192 x 8192 BF16 of 1 rank: walk 101, own 120 us; with
+// 8-bit outputs 118 and 132, of 3 ranks 201 and 232) - but not where a long launch has four destinations and more and a store is what
+// the wavefronts wait for (of 4 ranks 16384 x 8192: 649 and 593; of 8 ranks 8192 x 8192 624 and 576; 8192 x 6144 of 4 ranks 237 and 228; but 8192 x
+// 5120 of 5 ranks 265 and 291).  Of narrower rows a CU holds several, which overlap by themselves, and a launch of many has no
+// need of a walk (32768 x 2048 of 2 ranks 172 and 154, 65536 x 1024 of 1 rank 98 and 89, reduce_scatter of 8 ranks 2048 x 4096 258 and 234), one
+// of few has (1024 x 4096 of 2 ranks 10.9 and 12.4, 2048 x 4096 of 1 rank 13.7 and 14.8); nor have rows of one wavefront (65536 x 128 26 and 33).
+bool one_row_each(NormVariant v, uint32_t lanes, uint32_t nranks, uint32_t turns, bool stores_bound) {
+    if (lanes >= 768) return stores_bound;
+    return v == kNormBlock && lanes >= 128 && lanes <= (nranks == 1 ? 256u : 512u) && turns >= 8;
+}
+
+// Few rows: a CU would fold a row and store it to every destination while others idle.  Workgroups share the destinations
+// instead, up to 256 lanes for each CU, and each folds the row for itself, from the caches (8 ranks,
+// all of it by one workgroup and shared by eight, four, two: 1 x 8192 BF16 7.8 -> 6.3, 6.2, 6.8 us; 32 x 8192 8.3 -> 11.0, 7.4, 7.2; 64 x 4096
+// 5.5 -> 9.9, 6.8, 5.3; 32 x 2048 5.6 -> 4.9, 5.0, 5.2).  Not where a destination is an input: it would be read after it is written.
+constexpr uint32_t kSharedLanes = 65536;
+
+uint32_t shares(uint32_t ndst, uint64_t lanes) {
+    uint32_t n = 1;
+    while (2 * n <= ndst && 2 * n * lanes <= kSharedLanes) n *= 2;
+    return n;
+}
+
+// Of a buffer that an XCD writes in one run.  None, 64 KiB, 256 KiB, 1 MiB: 8192 x 8192 BF16 of 8 ranks, forward 601, 603, 577, 568 us, backward
+// 465, 439, 425, 420; 8192 x 4096 of 2 ranks 84.7, 83.7, 84.3, 84.6 and 75.1, 73.3, 73.2, 73.1; AdamW, 8 ranks, 98 M parameters, none and
+// 256 KiB: 1112 and 1043.
+constexpr uint32_t kDealBytes = 256 << 10;
 
 Deal deal_blocks(uint32_t blocks, uint64_t block_bytes) {
     Deal d{0, 0};
@@ -174,6 +213,8 @@ Deal deal_blocks(uint32_t blocks, uint64_t block_bytes) {
     return d;
 }
 
+// Whether rows may stream past the caches: then no line is written in two parts.  Streamed and through the caches: 8192 x 8192 BF16 of 8
+// ranks 577 and 617 us, backward 425 and 463, of 2 ranks 73 and 81; 1024 x 8192 of 8 ranks 76 and 90.
 bool on_lines(const std::vector<Rows>& buffers) {
     for (const Rows& b : buffers)
         if (b.at % 128 || (b.rows > 1 && b.stride % 128)) return false;
@@ -280,14 +321,10 @@ void NormPlan::plan_forward(int collective, const mrv_rms_norm_call& c) {
     L.positions = (s.rows + layout.each - 1) / layout.each;
     m_block = L.lanes = layout.lanes;
     const bool long_launch = written >= kLongBytes;
-    const bool one_each = v == kNormNarrow || v == kNormLong || (long_launch && L.ndst > 4);
-    m_grid = one_each ? L.positions : std::min(L.positions, resident(layout.lanes, s.nranks, s.stream32, false));
-    // Few rows: a CU would store a row to every destination while others idle (one row of 8192 to 8 ranks, hidden state and output:
-    // 256 KiB, 1.7 us at 64 bytes a clock).  Workgroups share the destinations instead, and read the row as often, from the caches.
-    // Not where a destination is an input: it would be read after it is written.
-    L.splits = 1;
-    if (v == kNormBlock && !in_place)
-        while (2 * L.splits <= L.ndst && 2 * L.splits * L.positions <= kComputeUnits) L.splits *= 2;
+    const uint32_t at_a_time = resident(layout.lanes, s.nranks, s.stream32, false);
+    const bool one_each = v == kNormNarrow || v == kNormLong || one_row_each(v, layout.lanes, s.nranks, L.positions / at_a_time, long_launch && L.ndst >= 4 && !q8);
+    m_grid = one_each ? L.positions : std::min(L.positions, at_a_time);
+    L.splits = v == kNormBlock && !in_place ? shares(L.ndst, uint64_t(L.positions) * layout.lanes) : 1;
     m_grid *= L.splits;
     L.deal = deal_blocks(L.positions, layout.each * L.send_stride);
     L.pace.on = long_launch && L.ndst > 1;

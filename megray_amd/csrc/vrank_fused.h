@@ -133,11 +133,16 @@ const void* norm_weight_kernel();  // grid: 64 columns each, parts
 // ---- AdamW over many tensors -------------------------------------------------------------------
 
 constexpr uint32_t kAdamVec = 8;               // elements of a lane
+// Lanes of a workgroup: a large one reads and writes longer runs of a buffer at a time, a small one is sooner done with its chain
+// of loads, scales and stores.  256 and 1024, BF16: the step with 32-bit states, 8 ranks, 98 M parameters 1088 and 1052 us, 1 rank, 157 M 766
+// and 737 (but 1 rank, 13 M, 60.1 and 62.4); with 8-bit states, 4 ranks, 50 M, 274 and 309; the norm, 8 ranks, 98 M, 236 and 261.
 constexpr uint32_t kAdamThreads = 1024;        // of the step with 32-bit states
 constexpr uint32_t kAdamThreads8 = 256;        // of the step with 8-bit states
 constexpr uint32_t kAdamNormThreads = 256;     // of the gradient norm
 constexpr uint32_t kAdamBlock = 256;                       // elements that share a scale of an 8-bit state: half a wavefront's
-constexpr uint32_t kAdamNormGroups = 512;                  // workgroups of the gradient norm, at most
+// Workgroups of the gradient norm, at most.  256, 512, 1024, 2048: 98 M BF16 of 8 ranks 323, 236, 247, 245 us; 0.8 M FP32 of 4 ranks 7.5, 7.2,
+// 7.2, 7.2.
+constexpr uint32_t kAdamNormGroups = 512;
 
 struct AdamTensor {  // one per tensor, in device memory
     uint64_t len;

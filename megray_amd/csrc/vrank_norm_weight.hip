@@ -1,4 +1,5 @@
-// Second launch of the norm's backward: the weight's gradient from the row groups' shares (vrank_fused.h).
+// Second launch of the norm's backward: the weight's gradient from the row groups' shares (vrank_fused.h).  Short, and bound by the
+// latency of its loads: eight in flight to a lane, a line and a half of a share to a wavefront; 3.4 us for 64 shares of 2048 columns.
 #include "vrank_fused_impl.hpp"
 
 namespace MegRay {
