@@ -392,7 +392,7 @@ enum {
  * out_dtype: dtype, or INT8 / MRV_FLOAT8_E4M3: then scales[r] (one float per row of outs[r]) get
  *   max(max |y|, 2^-100) / Q over the row and outs round(y / scale) to nearest even, Q = 127 / 448; a row with a value that is not
  *   finite gets the scale NaN and the codes 0 / NaN.
- * Strides are elements from one row to the next, 0 for cols.  cols >= 1; rows may be 0.
+ * Strides are elements from one row to the next, 0 for cols.  cols in [1, 2^26]; fewer than 2^22 rows of the fold, which may be 0.
  * outs[r] may be sendbuffs[r] (reduce_scatter: the place of rank r's own rows in it) and residual_outs[r] may be residuals[r] (all_reduce: residuals[0], for one r).
  */
 typedef struct mrv_rms_norm_call {

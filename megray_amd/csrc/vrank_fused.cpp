@@ -93,7 +93,7 @@ void check_collective(int collective, uint32_t nranks) {
 // Rows of the fold and row lengths that the launches count in 32 bits (grids in lanes, too).
 void check_extent(uint64_t rows, uint64_t cols) {
     if (cols < 1) MEGRAY_THROW("a row needs at least one element");
-    if (cols > (uint64_t(1) << 30)) MEGRAY_THROW("a row is too long");
+    if (cols > (uint64_t(1) << 26)) MEGRAY_THROW("a row is too long");
     if (rows >= (uint64_t(1) << 22)) MEGRAY_THROW("too many rows");
 }
 
@@ -384,6 +384,7 @@ void NormPlan::plan_backward(int collective, const mrv_rms_norm_backward_call& c
     const uint32_t nparts = s.gathered ? 1 : s.nranks;
     const uint32_t part_groups = backward_groups(v, s.cols, s.part_rows, s.nranks, nparts);
     uint64_t written = 0;
+    bool replaced_arriving = false;
     for (uint32_t r = 0; r < s.nranks; ++r) {
         const int own = int(s.gathered ? 0 : r);
         if (c.residual_out_grads && s.rows) {
@@ -393,6 +394,7 @@ void NormPlan::plan_backward(int collective, const mrv_rms_norm_backward_call& c
             rows.push_back(outputs.back());
             // in the hidden state's place, or in the arriving gradient's
             const bool arriving = c.residual_grads && L.dhidden[r] == L.arriving[own];
+            replaced_arriving |= arriving;
             replaces.push_back(int(s.nranks) + (arriving ? int(copies) : 0) + own);
             written += uint64_t(s.part_rows) * s.cols * s.stream_elem;
         }
@@ -439,8 +441,11 @@ void NormPlan::plan_backward(int collective, const mrv_rms_norm_backward_call& c
     L.weight32 = s.weight32;
     L.keep = written <= kKeepMaxBytes;
     L.eps = c.eps;
-    const Layout layout = norm_layout(v, s.cols);
-    m_first = kernels_for(c.dtype, v, s.nranks, s.stream32, on_lines(rows), false).backward;
+    // Two vectors per lane read the arriving gradient between their stores.  Where it is replaced and rows end inside a vector, the sweep
+    // takes the row groups instead: it reads and stores every element in one lane.
+    const NormVariant taken = v == kNormBlock2 && replaced_arriving && s.cols % kNormVec ? kNormLong : v;
+    const Layout layout = norm_layout(taken, s.cols);
+    m_first = kernels_for(c.dtype, taken, s.nranks, s.stream32, on_lines(rows), false).backward;
     m_grid = (L.groups + layout.each - 1) / layout.each;
     m_block = L.lanes = layout.lanes;
     L.deal = deal_blocks(v == kNormWave ? 0 : s.part_rows, L.send_stride);

@@ -365,7 +365,8 @@ __global__ void __launch_bounds__(Wave ? 64 * kWaveRows : 1024, 4) rms_norm_back
     const ConstBytes arriving_part = bytes_of(L.arriving[0] ? L.arriving[first] : nullptr);
 
     // As in the forward kernel the next row's loads are issued before this one's stores; two vectors per lane leave
-    // no registers for that, nor for the weight, which is read again where it is used.
+    // no registers for that, nor for the weight and the arriving gradient, which are read where they are used: the gradient may not be
+    // replaced then where a lane repeats elements of another, which may be stored by that time (NormPlan::plan_backward).
     FirstRanks<T, Lines, Vecs, Ranks> ahead;
     constexpr bool kArrivingAhead = kAhead && sizeof(R) == 2 && Ranks < 8;
     Raw8<R> hidden[Vecs], arriving[Vecs], arriving_ahead[Vecs];

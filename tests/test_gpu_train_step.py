@@ -287,6 +287,37 @@ def test_long_launches(n, rows, cols):
     assert bool(((dw[0].double() - exact).abs() <= 256 * U * size).all())
 
 
+@pytest.mark.parametrize("cols", [8192 + 1, 8192 + 5, 8200, 9221, 12293, 16383])
+@pytest.mark.parametrize("stream", [FP16, FP32])
+def test_wide_rows_in_place_of_the_arriving_gradient(cols, stream):
+    """Rows of two vectors per lane whose last vector overlaps another wavefront's (8193: the first lane of the eighth wavefront ends the row):
+    the gradient in the arriving one's place is, bit for bit or within the sums' order, the one beside it."""
+    n, rows = 2, 700
+    g = torch.Generator(device=DEV).manual_seed(cols)
+    t = torch.float32 if stream == FP32 else torch.float16
+    sends, weight = [randn(g, rows, cols).half() for _ in range(n)], randn(g, cols).half()
+    hidden, arriving = randn(g, rows, cols).to(t), randn(g, rows, cols).to(t)
+    space = torch.empty(mr.rms_norm_backward_workspace(AR, n, rows, cols), dtype=torch.uint8, device=DEV)
+    results = []
+    for place in (torch.empty_like(arriving), arriving.clone()):
+        source = place if results else arriving
+        dh, dw = [place, torch.empty_like(place)], [torch.empty(cols, device=DEV) for _ in range(n)]
+        mr.all_reduce_rms_norm_backward(sends, [hidden], weight, dh, rows, cols, FP16, EPS, residual_dtype=stream, residual_grads=[source],
+                                        weight_grads=dw, workspace=space)
+        torch.cuda.synchronize()
+        assert torch.equal(dh[0], dh[1])
+        results.append((dh[0].double(), dw[0].double()))
+    (beside, dw_beside), (over, dw_over) = results
+    # the two kernels add a row's terms in another order: their sums differ by fewer than 2 * 80 U of the terms' magnitudes
+    r = torch.rsqrt((hidden.double() ** 2).mean(-1, keepdim=True) + EPS)
+    size = sum(s.double().abs() for s in sends) * weight.double().abs()
+    near = 160 * U * (r * size + (hidden.double().abs() * r) * r * (size * hidden.double().abs() * r).mean(-1, keepdim=True) + arriving.double().abs())
+    step = 2 * torch.finfo(t).eps / 2
+    assert bool(((over - beside).abs() <= step * torch.maximum(over.abs(), beside.abs()) + near + torch.finfo(t).smallest_normal * step).all())
+    total = (sum(s.double().abs() for s in sends) * hidden.double().abs() * r).sum(0)
+    assert bool(((dw_over - dw_beside).abs() <= 512 * U * total).all())
+
+
 def test_two_plans_at_once():
     """Two backwards with a workspace each and two optimizers with an `out` each, on two streams at the same time."""
     n, rows, cols = 2, 900, 1024

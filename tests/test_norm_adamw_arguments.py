@@ -97,6 +97,7 @@ def test_what_both_directions_refuse(make):
     refused(make, "the weight's dtype", dtype=F32, weight_dtype=F16)
     refused(make, "at least one element", cols=0)
     refused(make, "too long", cols=1 << 31, rows=1)
+    refused(make, "too long", cols=(1 << 26) + 1, rows=1)  # a grid of the second launch counts lanes in 32 bits
     refused(make, "too many rows", rows=1 << 22)
     refused(make, "too many rows", rows=-1)
     refused(make, "too many rows", collective=RS, n=32, rows=1 << 20)
