@@ -229,6 +229,13 @@ NormKernels kernels_for(int dtype, NormVariant v, uint32_t nranks, bool stream32
     }
 }
 
+// Columns of a workgroup of the weight gradient's launch: few make many workgroups, many read whole lines of the shares.  64 and 16, both launches
+// together: 5099 x 88 of 8 ranks 22.1 and 17.7 us, 40000 x 256 of 1 rank 41.6 and 37.4, 65536 x 1024 117.6 and 114.6, 8192 x 4096 57.5 and 58.6,
+// 8192 x 8192 120 and 124, 4096 x 16384 of 4 ranks 249 and 259.
+uint32_t weight_cols(uint32_t cols) {
+    return cols < 4096 ? 16 : 64;
+}
+
 Status launch_kernel(const void* kernel, dim3 grid, uint32_t block, const void* descriptor, hipStream_t stream) {
     if (!grid.x) return MEGRAY_OK;
     void* args[] = {const_cast<void*>(descriptor)};
@@ -427,7 +434,8 @@ void NormPlan::plan_backward(int collective, const mrv_rms_norm_backward_call& c
         m_weight.cols = s.cols;
         m_weight.nparts = nparts;
         m_weight.nranks = s.nranks;
-        m_second = norm_weight_kernel();
+        m_weight_cols = weight_cols(s.cols);
+        m_second = norm_weight_kernel(m_weight_cols);
     }
     check_rows(outputs, replaces, inputs, replaced);
     if (!s.rows) return;  // the weight gradients are zero then
@@ -458,7 +466,7 @@ Status NormPlan::launch(hipStream_t stream) const {
         if (st != MEGRAY_OK) return st;
     }
     if (m_second)
-        return launch_kernel(m_second, dim3((m_weight.cols + 63) / 64, m_weight.nparts), kNormWeightThreads, &m_weight, stream);
+        return launch_kernel(m_second, dim3((m_weight.cols + m_weight_cols - 1) / m_weight_cols, m_weight.nparts), kNormWeightThreads, &m_weight, stream);
     return MEGRAY_OK;
 }
 

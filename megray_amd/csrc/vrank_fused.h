@@ -128,7 +128,7 @@ NormKernels norm_kernels_bf16(NormVariant v, uint32_t nranks, bool lines, bool q
 NormKernels norm_kernels_bf16_f32(NormVariant v, uint32_t nranks, bool lines, bool q8);
 NormKernels norm_kernels_f32(NormVariant v, uint32_t nranks, bool lines, bool q8);
 constexpr uint32_t kNormWeightThreads = 1024;
-const void* norm_weight_kernel();  // grid: 64 columns each, parts
+const void* norm_weight_kernel(uint32_t cols);  // of a workgroup, 16 or 64; grid: workgroups along a row, parts
 
 // ---- AdamW over many tensors -------------------------------------------------------------------
 
@@ -217,7 +217,7 @@ private:
     const void* m_first = nullptr;
     const void* m_second = nullptr;
     const void* m_descriptor = nullptr;  // of the first launch: m_forward or m_backward
-    uint32_t m_grid = 0, m_block = 0;
+    uint32_t m_grid = 0, m_block = 0, m_weight_cols = 0;
     NormLaunch m_forward;
     NormBackLaunch m_backward;
     NormWeightLaunch m_weight;

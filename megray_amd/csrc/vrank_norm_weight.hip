@@ -1,5 +1,5 @@
-// Second launch of the norm's backward: the weight's gradient from the row groups' shares (vrank_fused.h).  Short, and bound by the
-// latency of its loads: eight in flight to a lane, a line and a half of a share to a wavefront; 3.4 us for 64 shares of 2048 columns.
+// Second launch of the norm's backward: the weight's gradient from the row groups' shares (vrank_fused.h).  Short, and bound by the latency of
+// its loads, eight in flight to a lane: 3.6 us for 64 shares of 2048 columns, 5.0 for 512 of 8192 (16 MiB).
 #include "vrank_fused_impl.hpp"
 
 namespace MegRay {
@@ -9,24 +9,24 @@ namespace {
 
 using namespace fused;
 
-constexpr uint32_t kWaves = kNormWeightThreads / 64;
-
-// A workgroup takes 64 columns of one part, a lane each; its wavefronts split the part's row groups and meet in LDS.
-__global__ void __launch_bounds__(64 * kWaves) norm_weight(const NormWeightLaunch L) {
-    __shared__ float share[kWaves][64];
-    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const uint32_t col = blockIdx.x * 64 + lane, part = blockIdx.y;
+// A workgroup takes `Cols` columns of one part; its lanes take the part's row groups in turn, a column each, and meet in LDS.
+template <uint32_t Cols>
+__global__ void __launch_bounds__(kNormWeightThreads) norm_weight(const NormWeightLaunch L) {
+    constexpr uint32_t kTurns = kNormWeightThreads / Cols;
+    __shared__ float share[kTurns][Cols];
+    const uint32_t at = threadIdx.x % Cols, turn = threadIdx.x / Cols;
+    const uint32_t col = blockIdx.x * Cols + at, part = blockIdx.y;
     float sum = 0.0f;
     if (col < L.cols) {
         const float* p = L.partial + uint64_t(part) * L.part_groups * L.cols + col;
 #pragma unroll 8
-        for (uint32_t g = wave; g < L.part_groups; g += kWaves) sum += p[uint64_t(g) * L.cols];
+        for (uint32_t g = turn; g < L.part_groups; g += kTurns) sum += p[uint64_t(g) * L.cols];
     }
-    share[wave][lane] = sum;
+    share[turn][at] = sum;
     __syncthreads();
-    if (wave != 0 || col >= L.cols) return;
+    if (turn != 0 || col >= L.cols) return;
 #pragma unroll
-    for (uint32_t w = 1; w < kWaves; ++w) sum += share[w][lane];
+    for (uint32_t w = 1; w < kTurns; ++w) sum += share[w][at];
     if (L.nparts == 1)
         for (uint32_t r = 0; r < L.nranks; ++r) L.dweight[r][col] = sum;
     else
@@ -35,8 +35,8 @@ __global__ void __launch_bounds__(64 * kWaves) norm_weight(const NormWeightLaunc
 
 }  // namespace
 
-const void* norm_weight_kernel() {
-    return reinterpret_cast<const void*>(&norm_weight);
+const void* norm_weight_kernel(uint32_t cols) {
+    return cols == 16 ? reinterpret_cast<const void*>(&norm_weight<16>) : reinterpret_cast<const void*>(&norm_weight<64>);
 }
 
 }  // namespace vrank
