@@ -120,12 +120,15 @@ Shape check_shape(int collective, uint32_t nranks, size_t rows, size_t cols, int
 
 // ---- how a norm is laid out --------------------------------------------------------------------
 
-// A wavefront to a row up to 512 elements against a workgroup of one wavefront: 65536 x 128 BF16 of 8 ranks 163 and 187 us, 16384 x 509 of 8 ranks
+// A wavefront to a row up to 512 elements against a workgroup of one wavefront: 20000 x 384 BF16 of 8 ranks 77 and 79 us, 16384 x 509 of 8 ranks
 // 96 and 117, 40000 x 504 of 1 rank 31.5 and 32.6 (backward 51.4 and 51.8); at 512 itself they are level (24.4 and 24.6, 16384 rows of
 // 8 ranks 78 and 80, backward 75 and 66).  One vector per lane up to 8192 against two: 4096 x 8192 of 8 ranks 286 and 321 us, of 2 ranks 88 and
 // 104, backward 76 and 85.  Two up to 16384 against the row swept twice: 4096 x 16384 of 8 ranks 611 and 782, backward 467 and 744.
+// Sixteen lanes to a row up to 128 elements against a wavefront: 65536 x 64 BF16 of 1 rank 9.2 and 23.6 us, backward 16.6 and 43.4; 65536 x 128 of 8 ranks 93 and
+// 150, backward 78 and 77; 30000 x 127 of 2 ranks 11.5 and 18.7, backward 15.9 and 31.8 (FP32, 7000 x 99 of 4 ranks 10.1 and 8.7, backward 12.6 and 19.1).
 NormVariant norm_variant(uint32_t cols) {
     if (cols < kNormVec) return kNormNarrow;
+    if (cols <= 16 * kNormVec) return kNormShort;
     if (cols <= 64 * kNormVec) return kNormWave;
     if (cols <= 1024 * kNormVec) return kNormBlock;
     if (cols <= 2 * 1024 * kNormVec) return kNormBlock2;
@@ -137,10 +140,11 @@ struct Layout {
     uint32_t lanes, each;
 };
 
-Layout norm_layout(NormVariant v, uint32_t cols) {
+Layout norm_layout(NormVariant v, uint32_t cols, bool backward) {
     const uint32_t per_lane = v == kNormBlock2 ? 2 * kNormVec : kNormVec;
     switch (v) {
         case kNormNarrow: return {256, 256};
+        case kNormShort: return {256, backward ? 1u : 16u};
         case kNormWave: return {256, 4};
         case kNormLong: return {1024, 1};
         default: return {(cols + 64 * per_lane - 1) / (64 * per_lane) * 64, 1};
@@ -163,10 +167,11 @@ uint32_t resident(uint32_t lanes, uint32_t nranks, bool stream32, bool backward)
 // 422, 429 us, of 2 ranks 145 -> 145, 142; up to once and four times what the device holds: 427, 423, and 141, 145.)
 uint32_t backward_groups(NormVariant v, uint32_t cols, uint32_t part_rows, uint32_t nranks, uint32_t nparts) {
     if (!part_rows) return 0;
-    const Layout layout = norm_layout(v, cols);
+    const Layout layout = norm_layout(v, cols, true);
     uint32_t target = v == kNormNarrow ? 16384 : v == kNormLong ? kComputeUnits : resident(layout.lanes, nranks, false, true) * layout.each;
     target = std::max(1u, target / nparts);
-    if (v != kNormNarrow) target = std::min(std::max(target, part_rows / 16), 2 * target);
+    if (v == kNormShort) target = std::min(target, (part_rows + 31) / 32);  // two turns of a workgroup's sixteen rows
+    else if (v != kNormNarrow) target = std::min(std::max(target, part_rows / 16), 2 * target);
     const uint32_t each = (part_rows + target - 1) / target;
     return (part_rows + each - 1) / each;
 }
@@ -323,13 +328,13 @@ void NormPlan::plan_forward(int collective, const mrv_rms_norm_call& c) {
     L.has_hidden = c.residual_outs != nullptr;
     L.eps = c.eps;
     const NormVariant v = norm_variant(s.cols);
-    const Layout layout = norm_layout(v, s.cols);
+    const Layout layout = norm_layout(v, s.cols, false);
     m_first = kernels_for(c.dtype, v, s.nranks, s.stream32, on_lines(rows), q8).forward;
     L.positions = (s.rows + layout.each - 1) / layout.each;
     m_block = L.lanes = layout.lanes;
     const bool long_launch = written >= kLongBytes;
     const uint32_t at_a_time = resident(layout.lanes, s.nranks, s.stream32, false);
-    const bool one_each = v == kNormNarrow || v == kNormLong || one_row_each(v, layout.lanes, s.nranks, L.positions / at_a_time, long_launch && L.ndst >= 4 && !q8);
+    const bool one_each = v == kNormNarrow || v == kNormShort || v == kNormLong || one_row_each(v, layout.lanes, s.nranks, L.positions / at_a_time, long_launch && L.ndst >= 4 && !q8);
     m_grid = one_each ? L.positions : std::min(L.positions, at_a_time);
     L.splits = v == kNormBlock && !in_place ? shares(L.ndst, uint64_t(L.positions) * layout.lanes) : 1;
     m_grid *= L.splits;
@@ -452,11 +457,11 @@ void NormPlan::plan_backward(int collective, const mrv_rms_norm_backward_call& c
     // Two vectors per lane read the arriving gradient between their stores.  Where it is replaced and rows end inside a vector, the sweep
     // takes the row groups instead: it reads and stores every element in one lane.
     const NormVariant taken = v == kNormBlock2 && replaced_arriving && s.cols % kNormVec ? kNormLong : v;
-    const Layout layout = norm_layout(taken, s.cols);
+    const Layout layout = norm_layout(taken, s.cols, true);
     m_first = kernels_for(c.dtype, taken, s.nranks, s.stream32, on_lines(rows), false).backward;
     m_grid = (L.groups + layout.each - 1) / layout.each;
     m_block = L.lanes = layout.lanes;
-    L.deal = deal_blocks(v == kNormWave ? 0 : s.part_rows, L.send_stride);
+    L.deal = deal_blocks(v == kNormWave || v == kNormShort ? 0 : s.part_rows, L.send_stride);
     m_descriptor = &m_backward;
 }
 

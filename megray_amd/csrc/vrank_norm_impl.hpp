@@ -490,6 +490,132 @@ __global__ void __launch_bounds__(256) rms_norm_backward_narrow_kernel(const Nor
     }
 }
 
+// The fold of a lane's eight elements, for lanes whose rows differ.
+template <typename T, typename Part>
+__device__ __forceinline__ void short_fold(const void* const* send, uint32_t nranks, uint64_t row_offset, const Part& part, float (&acc)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
+#pragma unroll 8
+    for (uint32_t k = 0; k < nranks; ++k) {
+        float f[8];
+        widen<T>(part.template load<T, false>(bytes_of(send[k]) + row_offset, 0), f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] += f[i];
+    }
+}
+
+// Rows of up to 128 elements: sixteen lanes each, one row after the other in memory to a wavefront's four groups of lanes.  A wavefront for
+// such a row would leave three quarters of its lanes idle.
+constexpr uint32_t kShortLanes = 16;
+constexpr uint32_t kShortRows = 256 / kShortLanes;  // of a workgroup
+
+template <typename T, typename R, bool Q8>
+__global__ void __launch_bounds__(256) rms_norm_short_kernel(const NormLaunch L) {
+    const uint32_t lane = threadIdx.x % kShortLanes, row = L.deal.of(blockIdx.x) * kShortRows + threadIdx.x / kShortLanes;
+    if (row >= L.rows) return;  // all of a row's lanes or none
+    const uint32_t first = row / L.part_rows, at = row - first * L.part_rows;
+    const RowPart<1, false> part(L.cols, kShortLanes, lane);
+    float h[8], w[8], f[8];
+    Raw8<R> residual[1];
+    load_weight<T>(L.weight, L.weight32, part, 0, w);
+    load_row<R, false, 1>(bytes_of(L.residual[0] ? L.residual[first] : nullptr), uint64_t(at) * L.residual_stride, part, residual);
+    short_fold<T>(L.send, L.nranks, uint64_t(row) * L.send_stride, part, h);
+    widen<R>(residual[0], f);
+    float sum = 0.0f;
+    uint32_t top = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+        h[i] += f[i];
+        if (!part.mine(0, i)) continue;  // and lanes behind the row's end have none
+        sum = __builtin_fmaf(h[i], h[i], sum);
+        if (Q8) top = Larger()(top, magnitude(h[i] * w[i]));
+    }
+    sum = across_row(sum, Plus());
+    if (Q8) top = across_row(top, Larger());
+    const float r = 1.0f / __builtin_sqrtf(sum / float(L.cols) + L.eps);
+    float scale = 0.0f, inverse = 0.0f;
+    bool finite = true;
+    if (Q8) {
+        finite = row_scale(r, top, L.int8, scale, inverse);
+        if (lane == 0)
+            for (uint32_t d = 0; d < L.ndst; ++d) *(MRV_GLOBAL float*)(bytes_of(L.scales[first + d]) + uint64_t(at) * 4) = scale;
+    }
+    const Raw8<R> stored = narrow<R>(h);
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = h[i] * r * w[i];
+    Raw8<T> result;
+    if constexpr (Q8) {
+        const float limit = L.int8 ? kInt8Max : kE4m3Max;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = clamp_to(quotient(y[i], scale, inverse), limit);
+        u32x2 codes = L.int8 ? to_int8(y) : to_e4m3(y);
+        if (!finite) codes = L.int8 ? u32x2{0, 0} : u32x2{0x7f7f7f7fu, 0x7f7f7f7fu};
+        result.w[0] = codes[0], result.w[1] = codes[1];
+    } else {
+        result = narrow<T>(y);
+    }
+    for (uint32_t d = 0; d < L.ndst; ++d) {
+        if (L.has_hidden) part.template store<sizeof(R), false>(bytes_of(L.hidden[first + d]) + uint64_t(at) * L.hidden_stride, 0, stored.w, true);
+        part.template store<Q8 ? 1 : sizeof(T), false>(bytes_of(L.out[first + d]) + uint64_t(at) * L.out_stride, 0, result.w, true);
+    }
+}
+
+// Its backward: a workgroup is a row group, whose sixteen rows at a time add their shares of the weight's gradient up in LDS at the end.
+template <typename T, typename R>
+__global__ void __launch_bounds__(256) rms_norm_backward_short_kernel(const NormBackLaunch L) {
+    __shared__ float share[kShortRows][kShortLanes * kNormVec];
+    const uint32_t lane = threadIdx.x % kShortLanes, slot = threadIdx.x / kShortLanes;
+    const uint32_t first = blockIdx.x / L.part_groups;
+    const RowPart<1, false> part(L.cols, kShortLanes, lane);
+    float w[8], dw[8];
+    load_weight<T>(L.weight, L.weight32, part, 0, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dw[i] = 0.0f;
+    const ConstBytes hidden_part = bytes_of(L.hidden[first]), arriving_part = bytes_of(L.arriving[0] ? L.arriving[first] : nullptr);
+    for (uint32_t at = (blockIdx.x - first * L.part_groups) * kShortRows + slot; at < L.part_rows; at += L.part_groups * kShortRows) {
+        float g[8], h[8], dh[8];
+        Raw8<R> hidden[1], arriving[1];
+        load_row<R, false, 1>(hidden_part, uint64_t(at) * L.hidden_stride, part, hidden);
+        load_row<R, false, 1>(arriving_part, uint64_t(at) * L.arriving_stride, part, arriving);
+        short_fold<T>(L.send, L.nranks, (uint64_t(first) * L.part_rows + at) * L.send_stride, part, g);
+        widen<R>(hidden[0], h);
+        widen<R>(arriving[0], dh);
+        float square = 0.0f, inner = 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            if (!part.mine(0, i)) continue;
+            square = __builtin_fmaf(h[i], h[i], square);
+            inner = __builtin_fmaf(g[i] * w[i], h[i], inner);
+        }
+        square = across_row(square, Plus());
+        inner = across_row(inner, Plus());
+        const float r = 1.0f / __builtin_sqrtf(square / float(L.cols) + L.eps);
+        const float pull = r * r * r * (inner * (1.0f / float(L.cols)));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            dh[i] += __builtin_fmaf(-pull, h[i], r * (g[i] * w[i]));
+            dw[i] = __builtin_fmaf(g[i], h[i] * r, dw[i]);
+        }
+        const Raw8<R> wide = narrow<R>(dh);
+        const Raw8<T> slim = narrow<T>(dh);
+        for (uint32_t d = 0; d < L.ndst; ++d) {
+            if (L.dhidden[0]) part.template store<sizeof(R), false>(bytes_of(L.dhidden[first + d]) + uint64_t(at) * L.dhidden_stride, 0, wide.w, true);
+            if (L.dsend[0]) part.template store<sizeof(T), false>(bytes_of(L.dsend[first + d]) + uint64_t(at) * L.dsend_stride, 0, slim.w, true);
+        }
+    }
+    if (!L.partial) return;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i)
+        if (part.mine(0, i)) share[slot][part.col[0][0] + i] = dw[i];
+    __syncthreads();
+    if (threadIdx.x >= L.cols) return;
+    float sum = share[0][threadIdx.x];
+#pragma unroll
+    for (uint32_t s = 1; s < kShortRows; ++s) sum += share[s][threadIdx.x];
+    L.partial[uint64_t(blockIdx.x) * L.cols + threadIdx.x] = sum;
+}
+
 // Rows longer than the widest variant holds: the lanes sweep the row twice, the second time over data that the last-level
 // cache mostly still has.  The vector at the row's end is taken element by element, so no element is read after another
 // lane may have replaced it.
@@ -674,6 +800,10 @@ NormKernels norm_kernels_for(NormVariant v, uint32_t nranks, bool lines, bool q8
             return {q8 ? reinterpret_cast<const void*>(&rms_norm_narrow_kernel<T, R, true>)
                        : reinterpret_cast<const void*>(&rms_norm_narrow_kernel<T, R, false>),
                     reinterpret_cast<const void*>(&rms_norm_backward_narrow_kernel<T, R>)};
+        case kNormShort:
+            return {q8 ? reinterpret_cast<const void*>(&rms_norm_short_kernel<T, R, true>)
+                       : reinterpret_cast<const void*>(&rms_norm_short_kernel<T, R, false>),
+                    reinterpret_cast<const void*>(&rms_norm_backward_short_kernel<T, R>)};
         case kNormWave:
         case kNormBlock:
         case kNormBlock2: return lines ? norm_kernels_lines<T, R, true>(v, nranks, q8) : norm_kernels_lines<T, R, false>(v, nranks, q8);
