@@ -126,9 +126,13 @@ Shape check_shape(int collective, uint32_t nranks, size_t rows, size_t cols, int
 // 104, backward 76 and 85.  Two up to 16384 against the row swept twice: 4096 x 16384 of 8 ranks 611 and 782, backward 467 and 744.
 // Sixteen lanes to a row up to 128 elements against a wavefront: 65536 x 64 BF16 of 1 rank 9.2 and 23.6 us, backward 16.6 and 43.4; 65536 x 128 of 8 ranks 93 and
 // 150, backward 78 and 77; 30000 x 127 of 2 ranks 11.5 and 18.7, backward 15.9 and 31.8 (FP32, 7000 x 99 of 4 ranks 10.1 and 8.7, backward 12.6 and 19.1).
-NormVariant norm_variant(uint32_t cols) {
+// Thirty-two lanes to a row up to 256 and the workgroup's shares added in LDS against a wavefront and a share of each: backward of 65536 x 256 BF16 of 1 rank 33.9 and
+// 50.4 us, 16384 x 256 of 8 ranks 37.7 and 40.3, 20000 x 130 of 4 ranks 18.2 and 26.7 (forward of 8 ranks 44.9 and 36.2, of 1 rank 22.7 and 28.5;
+// a wavefront's lanes with the shares in LDS, up to 512: 16384 x 512 of 8 ranks 77.7 and 72.7, 16384 x 509 76.1 and 84.1).
+NormVariant norm_variant(uint32_t cols, bool backward) {
     if (cols < kNormVec) return kNormNarrow;
     if (cols <= 16 * kNormVec) return kNormShort;
+    if (cols <= 32 * kNormVec && backward) return kNormShort32;
     if (cols <= 64 * kNormVec) return kNormWave;
     if (cols <= 1024 * kNormVec) return kNormBlock;
     if (cols <= 2 * 1024 * kNormVec) return kNormBlock2;
@@ -145,6 +149,7 @@ Layout norm_layout(NormVariant v, uint32_t cols, bool backward) {
     switch (v) {
         case kNormNarrow: return {256, 256};
         case kNormShort: return {256, backward ? 1u : 16u};
+        case kNormShort32: return {256, 1};
         case kNormWave: return {256, 4};
         case kNormLong: return {1024, 1};
         default: return {(cols + 64 * per_lane - 1) / (64 * per_lane) * 64, 1};
@@ -170,7 +175,8 @@ uint32_t backward_groups(NormVariant v, uint32_t cols, uint32_t part_rows, uint3
     const Layout layout = norm_layout(v, cols, true);
     uint32_t target = v == kNormNarrow ? 16384 : v == kNormLong ? kComputeUnits : resident(layout.lanes, nranks, false, true) * layout.each;
     target = std::max(1u, target / nparts);
-    if (v == kNormShort) target = std::min(target, (part_rows + 31) / 32);  // two turns of a workgroup's sixteen rows
+    const uint32_t rows_at_a_time = v == kNormShort ? 16 : 8;
+    if (v == kNormShort || v == kNormShort32) target = std::min(target, (part_rows + 2 * rows_at_a_time - 1) / (2 * rows_at_a_time));
     else if (v != kNormNarrow) target = std::min(std::max(target, part_rows / 16), 2 * target);
     const uint32_t each = (part_rows + target - 1) / target;
     return (part_rows + each - 1) / each;
@@ -327,7 +333,7 @@ void NormPlan::plan_forward(int collective, const mrv_rms_norm_call& c) {
     L.keep = written <= kKeepMaxBytes;
     L.has_hidden = c.residual_outs != nullptr;
     L.eps = c.eps;
-    const NormVariant v = norm_variant(s.cols);
+    const NormVariant v = norm_variant(s.cols, false);
     const Layout layout = norm_layout(v, s.cols, false);
     m_first = kernels_for(c.dtype, v, s.nranks, s.stream32, on_lines(rows), q8).forward;
     L.positions = (s.rows + layout.each - 1) / layout.each;
@@ -348,7 +354,7 @@ size_t norm_backward_workspace(int collective, uint32_t nranks, size_t rows, siz
     const uint32_t nparts = collective == MRV_ALL_REDUCE ? 1 : nranks;
     if (rows >= (uint64_t(1) << 22)) MEGRAY_THROW("too many rows");
     check_extent(uint64_t(rows) * nparts, cols);
-    return size_t(backward_groups(norm_variant(uint32_t(cols)), uint32_t(cols), uint32_t(rows), nranks, nparts)) * nparts * cols * sizeof(float);
+    return size_t(backward_groups(norm_variant(uint32_t(cols), true), uint32_t(cols), uint32_t(rows), nranks, nparts)) * nparts * cols * sizeof(float);
 }
 
 void NormPlan::plan_backward(int collective, const mrv_rms_norm_backward_call& c) {
@@ -392,7 +398,7 @@ void NormPlan::plan_backward(int collective, const mrv_rms_norm_backward_call& c
         inputs.push_back({reinterpret_cast<uintptr_t>(c.weight), 1, uint64_t(s.cols) * (s.weight32 ? 4 : s.elem), 0, 0});
         replaced.push_back(inputs.back());
     }
-    const NormVariant v = norm_variant(s.cols);
+    const NormVariant v = norm_variant(s.cols, true);
     const uint32_t nparts = s.gathered ? 1 : s.nranks;
     const uint32_t part_groups = backward_groups(v, s.cols, s.part_rows, s.nranks, nparts);
     uint64_t written = 0;
@@ -461,7 +467,7 @@ void NormPlan::plan_backward(int collective, const mrv_rms_norm_backward_call& c
     m_first = kernels_for(c.dtype, taken, s.nranks, s.stream32, on_lines(rows), false).backward;
     m_grid = (L.groups + layout.each - 1) / layout.each;
     m_block = L.lanes = layout.lanes;
-    L.deal = deal_blocks(v == kNormWave || v == kNormShort ? 0 : s.part_rows, L.send_stride);
+    L.deal = deal_blocks(v == kNormWave || v == kNormShort || v == kNormShort32 ? 0 : s.part_rows, L.send_stride);
     m_descriptor = &m_backward;
 }
 

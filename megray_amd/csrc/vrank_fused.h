@@ -111,10 +111,10 @@ struct NormWeightLaunch {  // the second launch of a backward: weight gradients 
     uint32_t nranks;
 };
 
-// How a row is spread over lanes: rows of fewer than eight elements have a lane each (kNormNarrow), rows of up to 128 sixteen lanes (kNormShort), of
-// up to 512 a wavefront (kNormWave), rows of up to 8192 and 16384 a workgroup of as many wavefronts as they fill with one and two vectors per lane
+// How a row is spread over lanes: rows of fewer than eight elements have a lane each (kNormNarrow), rows of up to 128 sixteen lanes (kNormShort), in
+// the backward of up to 256 thirty-two (kNormShort32), of up to 512 a wavefront (kNormWave), rows of up to 8192 and 16384 a workgroup of as many wavefronts as they fill with one and two vectors per lane
 // (kNormBlock, kNormBlock2), and longer ones are swept twice (kNormLong).
-enum NormVariant { kNormNarrow, kNormShort, kNormWave, kNormBlock, kNormBlock2, kNormLong };
+enum NormVariant { kNormNarrow, kNormShort, kNormShort32, kNormWave, kNormBlock, kNormBlock2, kNormLong };
 
 struct NormKernels {  // addresses usable with hipLaunchKernel; null where the type has no such form
     const void* forward;

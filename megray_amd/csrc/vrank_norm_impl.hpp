@@ -561,19 +561,21 @@ __global__ void __launch_bounds__(256) rms_norm_short_kernel(const NormLaunch L)
     }
 }
 
-// Its backward: a workgroup is a row group, whose sixteen rows at a time add their shares of the weight's gradient up in LDS at the end.
-template <typename T, typename R>
+// Backward of rows of 8 * Lanes elements (16 or 32 lanes): a workgroup is a row group, whose rows at a time add their shares of the weight's
+// gradient up in LDS at the end.
+template <typename T, typename R, uint32_t Lanes>
 __global__ void __launch_bounds__(256) rms_norm_backward_short_kernel(const NormBackLaunch L) {
-    __shared__ float share[kShortRows][kShortLanes * kNormVec];
-    const uint32_t lane = threadIdx.x % kShortLanes, slot = threadIdx.x / kShortLanes;
+    constexpr uint32_t kRows = 256 / Lanes;
+    __shared__ float share[kRows][Lanes * kNormVec];
+    const uint32_t lane = threadIdx.x % Lanes, slot = threadIdx.x / Lanes;
     const uint32_t first = blockIdx.x / L.part_groups;
-    const RowPart<1, false> part(L.cols, kShortLanes, lane);
+    const RowPart<1, false> part(L.cols, Lanes, lane);
     float w[8], dw[8];
     load_weight<T>(L.weight, L.weight32, part, 0, w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) dw[i] = 0.0f;
     const ConstBytes hidden_part = bytes_of(L.hidden[first]), arriving_part = bytes_of(L.arriving[0] ? L.arriving[first] : nullptr);
-    for (uint32_t at = (blockIdx.x - first * L.part_groups) * kShortRows + slot; at < L.part_rows; at += L.part_groups * kShortRows) {
+    for (uint32_t at = (blockIdx.x - first * L.part_groups) * kRows + slot; at < L.part_rows; at += L.part_groups * kRows) {
         float g[8], h[8], dh[8];
         Raw8<R> hidden[1], arriving[1];
         load_row<R, false, 1>(hidden_part, uint64_t(at) * L.hidden_stride, part, hidden);
@@ -590,6 +592,10 @@ __global__ void __launch_bounds__(256) rms_norm_backward_short_kernel(const Norm
         }
         square = across_row(square, Plus());
         inner = across_row(inner, Plus());
+        if (Lanes == 32) {
+            square += __shfl_xor(square, 16, 64);
+            inner += __shfl_xor(inner, 16, 64);
+        }
         const float r = 1.0f / __builtin_sqrtf(square / float(L.cols) + L.eps);
         const float pull = r * r * r * (inner * (1.0f / float(L.cols)));
 #pragma unroll
@@ -612,7 +618,7 @@ __global__ void __launch_bounds__(256) rms_norm_backward_short_kernel(const Norm
     if (threadIdx.x >= L.cols) return;
     float sum = share[0][threadIdx.x];
 #pragma unroll
-    for (uint32_t s = 1; s < kShortRows; ++s) sum += share[s][threadIdx.x];
+    for (uint32_t s = 1; s < kRows; ++s) sum += share[s][threadIdx.x];
     L.partial[uint64_t(blockIdx.x) * L.cols + threadIdx.x] = sum;
 }
 
@@ -803,7 +809,8 @@ NormKernels norm_kernels_for(NormVariant v, uint32_t nranks, bool lines, bool q8
         case kNormShort:
             return {q8 ? reinterpret_cast<const void*>(&rms_norm_short_kernel<T, R, true>)
                        : reinterpret_cast<const void*>(&rms_norm_short_kernel<T, R, false>),
-                    reinterpret_cast<const void*>(&rms_norm_backward_short_kernel<T, R>)};
+                    reinterpret_cast<const void*>(&rms_norm_backward_short_kernel<T, R, 16>)};
+        case kNormShort32: return {nullptr, reinterpret_cast<const void*>(&rms_norm_backward_short_kernel<T, R, 32>)};
         case kNormWave:
         case kNormBlock:
         case kNormBlock2: return lines ? norm_kernels_lines<T, R, true>(v, nranks, q8) : norm_kernels_lines<T, R, false>(v, nranks, q8);

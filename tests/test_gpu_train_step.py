@@ -318,6 +318,43 @@ def test_wide_rows_in_place_of_the_arriving_gradient(cols, stream):
     assert bool(((dw_over - dw_beside).abs() <= 512 * U * total).all())
 
 
+@pytest.mark.parametrize("cols", [8, 17, 88, 127, 128, 129, 136, 250, 255, 256, 257])
+@pytest.mark.parametrize("collective", [AR, RS])
+@pytest.mark.parametrize("rows", [1, 15, 33, 3000])
+def test_short_rows(cols, collective, rows):
+    """Rows that share a wavefront, and row groups whose shares of the weight's gradient meet before they are stored: against 64 bits, and
+    in place bit for bit."""
+    n = 3
+    g = torch.Generator(device=DEV).manual_seed(cols + rows)
+    total = rows if collective == AR else rows * n
+    copies = 1 if collective == AR else n
+    sends = [randn(g, total, cols).bfloat16() for _ in range(n)]
+    hidden, arriving = [[randn(g, rows, cols) for _ in range(copies)] for _ in range(2)]
+    weight = randn(g, cols)
+    space = torch.empty(mr.rms_norm_backward_workspace(collective, n, rows, cols), dtype=torch.uint8, device=DEV)
+    call = mr.all_reduce_rms_norm_backward if collective == AR else mr.reduce_scatter_rms_norm_backward
+    results = []
+    for in_place in (False, True):
+        h = [t.clone() for t in hidden]
+        dh = (h + [torch.empty_like(h[0]) for _ in range(n - copies)]) if in_place else [torch.empty(rows, cols, device=DEV) for _ in range(n)]
+        dw = [torch.empty(cols, device=DEV) for _ in range(n)]
+        call(sends, h, weight, dh, rows, cols, BF16, EPS, residual_dtype=FP32, weight_dtype=FP32, residual_grads=arriving, weight_grads=dw, workspace=space)
+        torch.cuda.synchronize()
+        results.append((dh, dw))
+    for a, b in zip(results[0][0] + results[0][1], results[1][0] + results[1][1]):
+        assert torch.equal(a, b)
+    grads, sizes = sum(s.double() for s in sends).view(copies, rows, cols), sum(s.double().abs() for s in sends).view(copies, rows, cols)
+    for c in range(copies):
+        h, w, grad, size = hidden[c].double(), weight.double(), grads[c], sizes[c] * weight.double().abs()
+        r = torch.rsqrt((h * h).mean(-1, keepdim=True) + EPS)
+        want = r * grad * w - h * r ** 3 * (grad * w * h).mean(-1, keepdim=True) + arriving[c].double()
+        near = 100 * U * (r * size + h.abs() * r ** 3 * (size * h.abs()).mean(-1, keepdim=True) + arriving[c].double().abs())
+        assert bool(((results[0][0][c].double() - want).abs() <= near).all())
+        dw, per = (grad * h * r).sum(0), (sizes[c] * (h * r).abs()).sum(0)
+        # a group's rows (3000 / 94 at most, 2 a turn), its sixteen slots and 94 groups in turn: fewer than 200 additions, the rows' values off by 80 U
+        assert bool(((results[0][1][c].double() - dw).abs() <= 300 * U * per).all())
+
+
 def test_two_plans_at_once():
     """Two backwards with a workspace each and two optimizers with an `out` each, on two streams at the same time."""
     n, rows, cols = 2, 900, 1024
