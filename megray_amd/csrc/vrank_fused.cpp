@@ -512,6 +512,18 @@ bool Taken::overlaps(uintptr_t begin, uintptr_t end) const {
     return next != m_runs.begin() && std::prev(next)->second > begin;  // the last run that begins before `end`
 }
 
+namespace {
+
+// Workgroups of the gradient norm.  Few bytes in flight to each, or a tile or few, want many of them; where a lane loads 16 bytes of an element at
+// once or more and all of its ranks together, the fewer keep closer together.  512 and 2048: BF16, 98 M of 1 rank 87 and 38 us, 79 M of 3 ranks 100 and 76, of 4
+// ranks 110 and 99, 39 M of 16 ranks 203 and 196, 14 M of 8 ranks 49.6 and 41.2; 98 M of 8 ranks 235 and 244, 25 M 62.4 and 65.4 (but 29 M
+// 80.7 and 78.2); FP32, 24 M of 4 ranks 58.9 and 60.6, 39 M of 8 ranks 185 and 189.
+uint32_t norm_groups(uint64_t tiles, uint32_t ranks, size_t elem) {
+    return tiles >= 8192 && ranks <= 8 && ranks * elem >= 16 ? 512 : uint32_t(std::min<uint64_t>(tiles, 2048));
+}
+
+}  // namespace
+
 Adamw::Adamw(const mrv_adamw_tensors& t) {
     if (t.grad_ranks < 1 || t.grad_ranks > kMaxRanks) MEGRAY_THROW("grad_ranks must be in [1, 32]");
     const size_t grad_elem = float_size(t.grad_dtype, "unknown gradient dtype");
@@ -605,7 +617,7 @@ Adamw::Adamw(const mrv_adamw_tensors& t) {
     for (const Interval& x : used) written += x.written ? x.end - x.begin : 0;
     m_step.keep = written <= kKeepMaxBytes;
     m_step.pace.on = !state8 && written >= kLongBytes;
-    m_groups = uint32_t(std::min<uint64_t>(norm_tiles, kAdamNormGroups));
+    m_groups = norm_groups(norm_tiles, t.grad_ranks, grad_elem);
     if (hipGetDevice(&m_device) != hipSuccess) {
         (void)hipGetLastError();
         throw HipFailure();

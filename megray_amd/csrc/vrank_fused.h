@@ -140,9 +140,6 @@ constexpr uint32_t kAdamThreads = 1024;        // of the step with 32-bit states
 constexpr uint32_t kAdamThreads8 = 256;        // of the step with 8-bit states
 constexpr uint32_t kAdamNormThreads = 256;     // of the gradient norm
 constexpr uint32_t kAdamBlock = 256;                       // elements that share a scale of an 8-bit state: half a wavefront's
-// Workgroups of the gradient norm, at most.  256, 512, 1024, 2048: 98 M BF16 of 8 ranks 323, 236, 247, 245 us; 0.8 M FP32 of 4 ranks 7.5, 7.2,
-// 7.2, 7.2.
-constexpr uint32_t kAdamNormGroups = 512;
 
 struct AdamTensor {  // one per tensor, in device memory
     uint64_t len;
