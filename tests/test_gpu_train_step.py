@@ -355,6 +355,40 @@ def test_short_rows(cols, collective, rows):
         assert bool(((results[0][1][c].double() - dw).abs() <= 300 * U * per).all())
 
 
+@pytest.mark.parametrize("cols", [5, 100, 200, 500, 1000, 9000, 20000])
+def test_rows_four_gigabytes_apart(cols):
+    """Offsets past 32 bits: the third row begins 2^32 bytes and more behind the first, in every buffer; the results are those of rows beside each
+    other, bit for bit where the same kernel takes them."""
+    rows, stride = 3, (1 << 30) + 64
+    g = torch.Generator(device=DEV).manual_seed(cols)
+    far = [torch.empty(2 * stride + cols, dtype=torch.float16, device=DEV) for _ in range(4)]
+    rows_of = lambda t: [t[r * stride:r * stride + cols] for r in range(rows)]  # noqa: E731
+    near = [randn(g, rows, cols).half() for _ in range(2)]
+    weight = randn(g, cols).half()
+    for t, x in zip(far, near):
+        for r, v in enumerate(rows_of(t)):
+            v.copy_(x[r])
+    out, h = torch.empty_like(near[0]), torch.empty_like(near[0])
+    mr.all_reduce_rms_norm([near[0]], [out], weight, rows, cols, FP16, EPS, residuals=[near[1]], residual_outs=[h])
+    mr.all_reduce_rms_norm([far[0]], [far[2]], weight, rows, cols, FP16, EPS, residuals=[far[1]], residual_outs=[far[3]], send_stride=stride,
+                           residual_stride=stride, residual_out_stride=stride, out_stride=stride)
+    torch.cuda.synchronize()
+    assert torch.equal(torch.stack(rows_of(far[3])), h)
+    got = torch.stack(rows_of(far[2])).double()
+    assert bool(((got - out.double()).abs() <= 2.0 ** -10 * out.double().abs() + 2.0 ** -24).all())  # a step, if a sum took another order
+    dh, dsend, dw = torch.empty_like(h), torch.empty_like(h), [torch.empty(cols, device=DEV) for _ in range(2)]
+    space = torch.empty(mr.rms_norm_backward_workspace(AR, 1, rows, cols), dtype=torch.uint8, device=DEV)
+    mr.all_reduce_rms_norm_backward([near[0]], [h], weight, [dh], rows, cols, FP16, EPS, send_grads=[dsend], weight_grads=dw[:1], workspace=space)
+    mr.all_reduce_rms_norm_backward([far[0]], [far[3]], weight, [far[1]], rows, cols, FP16, EPS, send_grads=[far[2]], weight_grads=dw[1:], workspace=space,
+                                    send_stride=stride, hidden_stride=stride, residual_out_grad_stride=stride, send_grad_stride=stride)
+    torch.cuda.synchronize()
+    size = dh.double().abs().amax()
+    for t, want in ((far[1], dh), (far[2], dsend)):
+        assert bool(((torch.stack(rows_of(t)).double() - want.double()).abs() <= 2.0 ** -10 * want.double().abs() + 200 * U * size + 2.0 ** -24).all())
+    # three rows' terms |g| * |h * r|, the second at most 20 (a normal value beside its row's root mean square), each off by at most 2 * 100 U
+    assert bool(((dw[0] - dw[1]).abs() <= 200 * U * 3 * near[0].float().abs().amax() * 20).all())
+
+
 def test_two_plans_at_once():
     """Two backwards with a workspace each and two optimizers with an `out` each, on two streams at the same time."""
     n, rows, cols = 2, 900, 1024
