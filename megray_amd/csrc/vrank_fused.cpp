@@ -225,10 +225,13 @@ Deal deal_blocks(uint32_t blocks, uint64_t block_bytes) {
 }
 
 // Whether rows may stream past the caches: then no line is written in two parts.  Streamed and through the caches: 8192 x 8192 BF16 of 8
-// ranks 577 and 617 us, backward 425 and 463, of 2 ranks 73 and 81; 1024 x 8192 of 8 ranks 76 and 90.
-bool on_lines(const std::vector<Rows>& buffers) {
+// ranks 577 and 617 us, backward 425 and 463, of 2 ranks 73 and 81; 1024 x 8192 of 8 ranks 76 and 90.  What streams leaves by buffer stores, which
+// need a 4-byte boundary: a stored row's last piece ends with the row, so the row has to end on one.
+bool on_lines(const std::vector<Rows>& buffers, const std::vector<Rows>& stored) {
     for (const Rows& b : buffers)
         if (b.at % 128 || (b.rows > 1 && b.stride % 128)) return false;
+    for (const Rows& b : stored)
+        if (b.bytes % 4) return false;
     return true;
 }
 
@@ -335,7 +338,7 @@ void NormPlan::plan_forward(int collective, const mrv_rms_norm_call& c) {
     L.eps = c.eps;
     const NormVariant v = norm_variant(s.cols, false);
     const Layout layout = norm_layout(v, s.cols, false);
-    m_first = kernels_for(c.dtype, v, s.nranks, s.stream32, on_lines(rows), q8).forward;
+    m_first = kernels_for(c.dtype, v, s.nranks, s.stream32, on_lines(rows, outputs), q8).forward;
     L.positions = (s.rows + layout.each - 1) / layout.each;
     m_block = L.lanes = layout.lanes;
     const bool long_launch = written >= kLongBytes;
@@ -464,7 +467,7 @@ void NormPlan::plan_backward(int collective, const mrv_rms_norm_backward_call& c
     // takes the row groups instead: it reads and stores every element in one lane.
     const NormVariant taken = v == kNormBlock2 && replaced_arriving && s.cols % kNormVec ? kNormLong : v;
     const Layout layout = norm_layout(taken, s.cols, true);
-    m_first = kernels_for(c.dtype, taken, s.nranks, s.stream32, on_lines(rows), false).backward;
+    m_first = kernels_for(c.dtype, taken, s.nranks, s.stream32, on_lines(rows, outputs), false).backward;
     m_grid = (L.groups + layout.each - 1) / layout.each;
     m_block = L.lanes = layout.lanes;
     L.deal = deal_blocks(v == kNormWave || v == kNormShort || v == kNormShort32 ? 0 : s.part_rows, L.send_stride);

@@ -121,7 +121,8 @@ struct NormKernels {  // addresses usable with hipLaunchKernel; null where the t
     const void* backward;
 };
 
-// in vrank_norm_<sends' type>[_<residual stream's type>].hip; `lines`: every row of every buffer begins on a cache line
+// in vrank_norm_<sends' type>[_<residual stream's type>].hip; `lines`: every row of every buffer begins on a cache line,
+// and every stored row ends on a 4-byte boundary
 NormKernels norm_kernels_f16(NormVariant v, uint32_t nranks, bool lines, bool q8);
 NormKernels norm_kernels_f16_f32(NormVariant v, uint32_t nranks, bool lines, bool q8);
 NormKernels norm_kernels_bf16(NormVariant v, uint32_t nranks, bool lines, bool q8);

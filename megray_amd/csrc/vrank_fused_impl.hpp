@@ -151,7 +151,7 @@ constexpr int kStream = 18;  // sc1 | nt
 constexpr int kStay = 16;    // sc1
 template <uint32_t Count, bool Lines, int Align>
 __device__ __forceinline__ void store_dwords(Bytes base, uint32_t offset, const uint32_t* w, bool keep) {
-    if constexpr (Lines) {  // `base` is the same for the whole wavefront
+    if constexpr (Lines) {  // `base` is the same for the whole wavefront, base + offset a multiple of four: what a buffer store needs
         const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, -1, 0x00020000);
         if constexpr (Count == 4) {
             if (keep) __builtin_amdgcn_raw_buffer_store_b32(int32_t(w[0]), rsrc, int(offset), 0, kStay);

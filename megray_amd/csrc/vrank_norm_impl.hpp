@@ -82,7 +82,8 @@ struct RowPart {
         if constexpr (Split) return load44<T, Once>(row + col[k][0] * uint32_t(sizeof(T)), row + col[k][kPieces - 1] * uint32_t(sizeof(T)));
         else return load8<T, Once>(row + col[k][0] * uint32_t(sizeof(T)));
     }
-    // `w`: the vector's eight elements, `Size` bytes each
+    // `w`: the vector's eight elements, `Size` bytes each.  Lines: a buffer store, whose offset has to be a multiple of four - that of a piece
+    // that is moved back, too, which is why the row has to end on one.
     template <uint32_t Size, bool Lines>
     __device__ __forceinline__ void store(Bytes row, uint32_t k, const uint32_t* w, bool keep) const {
 #pragma unroll
@@ -187,7 +188,7 @@ __device__ __forceinline__ bool row_scale(float r, uint32_t top, uint32_t int8, 
 }
 
 // R: the residual stream's type.  Q8: 8-bit output with a scale per row.  Wave: a row is one wavefront's.  Lines: every row of every
-// buffer begins on a cache line.
+// buffer begins on a cache line, and every stored row ends on a 4-byte boundary.
 template <typename T, typename R, bool Q8, uint32_t Vecs, bool Wave, bool Lines, uint32_t Ranks>
 __global__ void __launch_bounds__(Wave ? 64 * kWaveRows : 1024, 4) rms_norm_kernel(const NormLaunch L) {
     typedef RowReduce<Wave, 1, Q8> Reduce;
