@@ -342,6 +342,8 @@ __global__ void __launch_bounds__(256) rms_norm_narrow_kernel(const NormLaunch L
 
 // Backward.  A row group (the lanes of one row) walks the rows of one part, `part_groups` apart, and carries its columns'
 // share of the weight's gradient in registers; the shares meet in `partial`, and norm_weight_kernel adds them in order.
+// dh is formed as r * (g * w - h * pull), pull = r * (r * mean(g * w * h)): pull is of dh's size and h * pull of g * w's, so neither leaves the
+// range of 32 bits before dh does; r^3 would, from rows of 1e13 on and below 1e-13.
 template <typename T, typename R, uint32_t Vecs, bool Wave, bool Lines, uint32_t Ranks>
 __global__ void __launch_bounds__(Wave ? 64 * kWaveRows : 1024, 4) rms_norm_backward_kernel(const NormBackLaunch L) {
     typedef RowReduce<Wave, 2, false> Reduce;
@@ -408,7 +410,7 @@ __global__ void __launch_bounds__(Wave ? 64 * kWaveRows : 1024, 4) rms_norm_back
         uint32_t unused = 0;
         Reduce::run(shared, lanes / 64, slot, sum, unused);
         const float r = 1.0f / __builtin_sqrtf(sum[0] / float(L.cols) + L.eps);
-        const float pull = r * r * r * (sum[1] * mean);
+        const float pull = r * (r * (sum[1] * mean));
         const uint64_t dhidden_row = uint64_t(at) * L.dhidden_stride, dsend_row = uint64_t(at) * L.dsend_stride;
 #pragma unroll
         for (uint32_t k = 0; k < Vecs; ++k) {
@@ -418,7 +420,7 @@ __global__ void __launch_bounds__(Wave ? 64 * kWaveRows : 1024, 4) rms_norm_back
             else widen<R>(arriving_part ? part.template load<R, Lines>(arriving_part + uint64_t(at) * L.arriving_stride, k) : Raw8<R>{}, dh);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                dh[i] += __builtin_fmaf(-pull, h[k][i], r * (g[k][i] * w[k][i]));
+                dh[i] = __builtin_fmaf(r, __builtin_fmaf(-pull, h[k][i], g[k][i] * w[k][i]), dh[i]);
                 dw[k][i] = __builtin_fmaf(g[k][i], h[k][i] * r, dw[k][i]);
             }
             const Raw8<R> wide = narrow<R>(dh);
@@ -470,11 +472,11 @@ __global__ void __launch_bounds__(256) rms_norm_backward_narrow_kernel(const Nor
             inner = __builtin_fmaf(g[c] * w[c], h[c], inner);
         }
         const float r = 1.0f / __builtin_sqrtf(square / float(L.cols) + L.eps);
-        const float pull = r * r * r * (inner * (1.0f / float(L.cols)));
+        const float pull = r * (r * (inner * (1.0f / float(L.cols))));
 #pragma unroll
         for (uint32_t c = 0; c < kNormVec; ++c) {
             if (c >= L.cols) continue;
-            const float dh = a[c] + __builtin_fmaf(-pull, h[c], r * (g[c] * w[c]));
+            const float dh = __builtin_fmaf(r, __builtin_fmaf(-pull, h[c], g[c] * w[c]), a[c]);
             dw[c] = __builtin_fmaf(g[c], h[c] * r, dw[c]);
             for (uint32_t d = 0; d < L.ndst; ++d) {
                 if (L.dhidden[0])
@@ -598,10 +600,10 @@ __global__ void __launch_bounds__(256) rms_norm_backward_short_kernel(const Norm
             inner += __shfl_xor(inner, 16, 64);
         }
         const float r = 1.0f / __builtin_sqrtf(square / float(L.cols) + L.eps);
-        const float pull = r * r * r * (inner * (1.0f / float(L.cols)));
+        const float pull = r * (r * (inner * (1.0f / float(L.cols))));
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            dh[i] += __builtin_fmaf(-pull, h[i], r * (g[i] * w[i]));
+            dh[i] = __builtin_fmaf(r, __builtin_fmaf(-pull, h[i], g[i] * w[i]), dh[i]);
             dw[i] = __builtin_fmaf(g[i], h[i] * r, dw[i]);
         }
         const Raw8<R> wide = narrow<R>(dh);
@@ -758,7 +760,7 @@ __global__ void __launch_bounds__(kLongLanes) rms_norm_backward_long_kernel(cons
                 if (L.arriving[0])
                     load_part<R>(bytes_of(L.arriving[first]) + uint64_t(at) * L.arriving_stride + c * sizeof(R), have, dh);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) dh[i] += __builtin_fmaf(-pull, h[i], r * (g[i] * w[i]));
+                for (int i = 0; i < 8; ++i) dh[i] = __builtin_fmaf(r, __builtin_fmaf(-pull, h[i], g[i] * w[i]), dh[i]);
                 for (uint32_t d = 0; d < L.ndst; ++d) {
                     if (L.dhidden[0])
                         store_part<R>(bytes_of(L.dhidden[first + d]) + uint64_t(at) * L.dhidden_stride + c * sizeof(R), have, dh);
@@ -770,7 +772,7 @@ __global__ void __launch_bounds__(kLongLanes) rms_norm_backward_long_kernel(cons
             uint32_t unused = 0;
             Reduce::run(shared, kLongLanes / 64, slot, sum, unused);
             r = 1.0f / __builtin_sqrtf(sum[0] / float(L.cols) + L.eps);
-            pull = r * r * r * (sum[1] * (1.0f / float(L.cols)));
+            pull = r * (r * (sum[1] * (1.0f / float(L.cols))));
         }
     }
 }
