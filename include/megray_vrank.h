@@ -392,6 +392,8 @@ enum {
  * out_dtype: dtype, or INT8 / MRV_FLOAT8_E4M3: then scales[r] (one float per row of outs[r]) get
  *   max(max |y|, 2^-100) / Q over the row and outs round(y / scale) to nearest even, Q = 127 / 448; a row with a value that is not
  *   finite gets the scale NaN and the codes 0 / NaN.
+ * Squares are summed in 32 bits, like everything else: the formula holds while a row's sum of h * h is less than 2^128 (from there on
+ *   1 / sqrt is 0, and so is every finite element's y) and mean(h * h) + eps is at least 2^-110; with 8-bit outputs |h * weight| < 2^128, too.
  * Strides are elements from one row to the next, 0 for cols.  cols in [1, 2^26]; fewer than 2^22 rows of the fold, which may be 0.
  * outs[r] may be sendbuffs[r] (reduce_scatter: the place of rank r's own rows in it) and residual_outs[r] may be residuals[r] (all_reduce: residuals[0], for one r).
  */
@@ -416,7 +418,7 @@ MRV_API int mrv_rms_norm(int collective, const mrv_rms_norm_call* call, void* st
  * copy, entry 0 (all_reduce), or rank r's rows (reduce_scatter).  With g = sum over k of sendbuffs[k], r = 1 / sqrt(mean(h * h) + eps):
  *   dh = r * g * weight - h * r^3 * mean(g * weight * h) + residual_grad
  *   dweight = sum over rows of g * h * r
- * dh is the gradient of the residual and of every rank's sendbuff of the forward: it goes to residual_out_grads
+ * for the forward's range of h.  dh is the gradient of the residual and of every rank's sendbuff of the forward: it goes to residual_out_grads
  * (residual_dtype) and / or send_grads (dtype), either may be null, to every rank (all_reduce) or rank r's rows to rank r.
  * weight_grads (null: not wanted): `cols` floats per rank, over all rows (all_reduce) or the rank's own (reduce_scatter);
  * they need `workspace`, device memory of mrv_rms_norm_backward_workspace() bytes, aligned to 4 and not used by another call at the
@@ -462,8 +464,8 @@ MRV_API void mrv_norm_plan_destroy(mrv_norm_plan* plan);
  *   exp_avgs[t], exp_avg_sqs[t]: the running means m and v.  state_dtype FLOAT32: floats.  MRV_FLOAT8_E4M3: codes with
  *     a float scale for each 256 elements from the tensor's start (the last block may be shorter) in exp_avg_scales[t] and exp_avg_sq_scales[t]:
  *     scale = max(max |x|, 2^-100) / 448 over the block, code = round(x / scale); the second holds x = sqrt(v), and
- *     a value above zero gets at least the smallest code (2^-9), so that no denominator is lost.  Zeroed codes and scales are
- *     a valid beginning.
+ *     a value above zero gets at least the smallest code (2^-9), so that no denominator is lost; a block with a value that is
+ *     not finite gets the scale NaN and NaN codes, all of it.  Zeroed codes and scales are a valid beginning.
  *   weight_decays[t] (null: 0).
  * A handle without params (null) serves mrv_adamw_grad_norm alone.
  */
@@ -498,7 +500,7 @@ MRV_API int mrv_adamw_grad_norm(const mrv_adamw* handle, float grad_scale, float
  * One step, with g = grad_scale * *clip * sum over k of grads[k] (clip: a float in device memory, out + 1 of the call above say; null: 1):
  *   m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g g,
  *   p = p (1 - lr weight_decay) - lr (m / (1 - beta1^step)) / (sqrt(v / (1 - beta2^step)) + eps)
- * in 32 bits; params get p rounded to their type.  `clip` is not part of what the step writes.  A step whose *clip is not finite changes nothing.  `step` counts from 1.  The
+ * in 32 bits (a square past their range makes v infinite); params get p rounded to their type.  `clip` is not part of what the step writes.  A step whose *clip is not finite changes nothing.  `step` counts from 1.  The
  * numbers are arguments of the launch: a step captured into a graph repeats them.
  */
 typedef struct mrv_adamw_step_args {
