@@ -456,7 +456,8 @@ MRV_API void mrv_norm_plan_destroy(mrv_norm_plan* plan);
  * AdamW over many tensors at once, on gradients that are still apart: every rank's gradients are read and summed in
  * the step itself, and the new parameters are written to every rank.  mrv_adamw_create checks the tensors and keeps their addresses in
  * a table in device memory (it allocates and copies, synchronously); the tensors have to stay where they are until
- * mrv_adamw_destroy, which frees the table: no call on the handle may still be running then.
+ * mrv_adamw_destroy, which frees the table: no call on the handle may still be running then, and a graph into which one of its calls
+ * was captured may not be launched any more (its launches hold the table's address).  Neither may be called while a stream is being captured.
  *   grads[k * ntensors + t], params[k * ntensors + t]: rank k's tensor t, lens[t] elements of grad_dtype / param_dtype
  *     (FLOAT16, MRV_BFLOAT16, FLOAT32).  grad_ranks and param_ranks (1 .. 32) may differ: gradients that were reduced
  *     before have one rank.  lens[t] may be 0 (the pointers are not read then).

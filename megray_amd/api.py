@@ -495,7 +495,9 @@ class AdamWPlan:
     grads[r][t]: rank r's gradient of tensor t, lengths[t] elements of grad_dtype; params[r][t] likewise, written by step().
     masters[t]: the 32-bit parameters (None with FLOAT32 params: rank 0's are the masters).  exp_avgs, exp_avg_sqs: floats, or
     with state_dtype FLOAT8_E4M3 codes with a float for each 256 elements in exp_avg_scales[t], exp_avg_sq_scales[t].
-    Without params a plan has grad_norm() alone.  The tensors must outlive the plan, and stay where they are."""
+    Without params a plan has grad_norm() alone.  The tensors must outlive the plan, and stay where they are.  The plan owns a
+    table in device memory that its launches read: keep the plan as long as any graph into which its calls were captured; close(), and
+    the end of the last reference, free the table."""
 
     def __init__(self, grads, lengths, grad_dtype, params=None, param_dtype=None, masters=None, exp_avgs=None, exp_avg_sqs=None,
                  state_dtype=DType.FLOAT32, exp_avg_scales=None, exp_avg_sq_scales=None, weight_decays=None):
