@@ -247,7 +247,8 @@ __device__ __forceinline__ double workgroup_sum(double x) {
     return x;
 }
 
-// Squares are summed in 64 bits: no gradient that is finite in 32 bits overflows, and the number of terms does not matter.
+// Squares are summed in 64 bits: no gradient that is finite in 32 bits overflows, and the number of terms does not matter.  The gradients are loaded as
+// data that need not stay in the caches; the step that follows reads them again, of a large model (1.5 GB above) from memory either way.
 template <typename G>
 __global__ void __launch_bounds__(kAdamNormThreads) adamw_norm_kernel(const AdamNormLaunch L) {
     double sum = 0.0;

@@ -128,7 +128,8 @@ Shape check_shape(int collective, uint32_t nranks, size_t rows, size_t cols, int
 // 150, backward 78 and 77; 30000 x 127 of 2 ranks 11.5 and 18.7, backward 15.9 and 31.8 (FP32, 7000 x 99 of 4 ranks 10.1 and 8.7, backward 12.6 and 19.1).
 // Thirty-two lanes to a row up to 256 and the workgroup's shares added in LDS against a wavefront and a share of each: backward of 65536 x 256 BF16 of 1 rank 33.9 and
 // 50.4 us, 16384 x 256 of 8 ranks 37.7 and 40.3, 20000 x 130 of 4 ranks 18.2 and 26.7 (forward of 8 ranks 44.9 and 36.2, of 1 rank 22.7 and 28.5;
-// a wavefront's lanes with the shares in LDS, up to 512: 16384 x 512 of 8 ranks 77.7 and 72.7, 16384 x 509 76.1 and 84.1).
+// a wavefront's lanes with the shares in LDS, up to 512: 16384 x 512 of 8 ranks 77.7 and 72.7, 16384 x 509 76.1 and 84.1).  The rule knows widths alone; where
+// two figures of a width differ by rank count or type (256 forward, 99 of FP32) it takes what serves the wider range of the backward and the rank counts.
 NormVariant norm_variant(uint32_t cols, bool backward) {
     if (cols < kNormVec) return kNormNarrow;
     if (cols <= 16 * kNormVec) return kNormShort;
@@ -159,9 +160,11 @@ Layout norm_layout(NormVariant v, uint32_t cols, bool backward) {
 constexpr uint32_t kComputeUnits = 256;
 
 // Workgroups that the device holds at a time, by the registers of the kernels for so many ranks (norm_kernels_ranks in
-// vrank_norm_impl.hpp): a walk over rows with more of them than that would run its second half after its first.  (Twice as many and half
-// as many: 8192 x 8192 BF16 of 8 ranks, forward, 575 -> 579, 575 us, backward 423 -> 423, 424; 2048 x 4096 of 4 ranks 35.9 -> 36.2, 36.0, backward
-// 35.2 -> 39.6, 33.3.)
+// vrank_norm_impl.hpp): a walk over rows with more of them than that would run its second half after its first.  The least over the types with one vector per
+// lane: a CU holds 24 - 32 wavefronts of the forward for up to two ranks, 20 - 28 for up to four (16 - 24 with a 32-bit stream), 16 above; of the backward 20,
+// 16 - 20 and 16.  Two vectors per lane leave 16 (BF16's backward 20): rows of 8193 to at most 12288 elements of up to four ranks get twice the workgroups
+// that are held.  (Twice as many and half as many: 8192 x 8192 BF16 of 8 ranks, forward, 575 -> 579, 575 us, backward 423 -> 423, 424; 2048 x 4096 of 4
+// ranks 35.9 -> 36.2, 36.0, backward 35.2 -> 39.6, 33.3.)
 uint32_t resident(uint32_t lanes, uint32_t nranks, bool stream32, bool backward) {
     const uint32_t waves = backward ? (nranks <= 2 ? 20 : 16) : nranks <= 2 ? 24 : nranks <= 4 && !stream32 ? 20 : 16;
     return kComputeUnits * std::max(1u, waves * 64 / lanes);
@@ -169,7 +172,9 @@ uint32_t resident(uint32_t lanes, uint32_t nranks, bool stream32, bool backward)
 
 // Row groups of a backward, per part: enough to fill the device and no more than twice that, sixteen rows to each if there are (a group
 // writes its share of the weight's gradient once), as many to each as to the others.  (Eight rows to each and 32: 8192 x 8192 BF16 of 8 ranks 423 ->
-// 422, 429 us, of 2 ranks 145 -> 145, 142; up to once and four times what the device holds: 427, 423, and 141, 145.)
+// 422, 429 us, of 2 ranks 145 -> 145, 142; up to once and four times what the device holds: 427, 423, and 141, 145.  Half as many groups of up to 256 lanes:
+// 65536 x 1024 of 1 rank 113 -> 101, 8192 x 512 of 8 ranks 44.1 -> 39.2, 8192 x 1024 59.8 -> 55.5, 2000 x 2048 35.6 -> 33.1, 3000 x 300 of 2 ranks
+// 15.4 -> 12.5, but 16384 x 2048 of 1 rank 53.4 -> 56.3 and 20000 x 1500 of 4 ranks 128.3 -> 128.4; a quarter: 141, 39.7, 62.4, 35.5, 12.6, 74.5.)
 uint32_t backward_groups(NormVariant v, uint32_t cols, uint32_t part_rows, uint32_t nranks, uint32_t nparts) {
     if (!part_rows) return 0;
     const Layout layout = norm_layout(v, cols, true);
@@ -226,7 +231,8 @@ Deal deal_blocks(uint32_t blocks, uint64_t block_bytes) {
 
 // Whether rows may stream past the caches: then no line is written in two parts.  Streamed and through the caches: 8192 x 8192 BF16 of 8
 // ranks 577 and 617 us, backward 425 and 463, of 2 ranks 73 and 81; 1024 x 8192 of 8 ranks 76 and 90.  What streams leaves by buffer stores, which
-// need a 4-byte boundary: a stored row's last piece ends with the row, so the row has to end on one.
+// need a 4-byte boundary: a stored row's last piece ends with the row, so the row has to end on one.  BF16 rows of 4160 elements' distance, 4099 of them
+// used (through the caches) and 4100 (streamed): 8192 of 8 ranks 355 and 436, backward 257 and 232, of 1 rank 56 and 52, backward 100 and 93.
 bool on_lines(const std::vector<Rows>& buffers, const std::vector<Rows>& stored) {
     for (const Rows& b : buffers)
         if (b.at % 128 || (b.rows > 1 && b.stride % 128)) return false;

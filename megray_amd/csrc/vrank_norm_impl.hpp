@@ -7,8 +7,11 @@
 // stored to every destination from the registers.  The bound is HBM: two to four bytes of traffic per operation.
 //
 // A row whose length is no multiple of eight ends in a vector that is moved back to end with the row: the lane that owns
-// it repeats up to seven elements of its neighbour, leaves them out of the sums, and stores the same values.  All loads of a
-// row come before the reduction and all its stores behind it, so outputs that take an input's place are safe with that too.
+// it repeats up to seven elements of its neighbour, leaves them out of the sums, and stores the same values.  Where all loads of a
+// row come before the reduction and all its stores behind it, outputs that take an input's place are safe with that too.  Two kernels load
+// behind the reduction.  The backward with two vectors per lane reads the arriving gradient between its stores: it may not be replaced
+// where rows end inside a vector (NormPlan::plan_backward takes the sweep there).  The kernels that sweep a row twice read it again
+// as they store it: they move no vector back, and each element is read and stored by one lane alone.
 #pragma once
 
 #include "vrank_fused_impl.hpp"

@@ -1,5 +1,5 @@
 // Second launch of the norm's backward: the weight's gradient from the row groups' shares (vrank_fused.h).  Short, and bound by the latency of
-// its loads, eight in flight to a lane: 3.6 us for 64 shares of 2048 columns, 5.0 for 512 of 8192 (16 MiB).
+// its loads: 2.9 us for 64 shares of 2048 columns (one load to a lane, 128 workgroups), 4.9 for 512 of 8192 (16 MiB, 32 loads to a lane, eight in flight).
 #include "vrank_fused_impl.hpp"
 
 namespace MegRay {
